@@ -306,6 +306,143 @@ int tcb_llama_batch_capture(tcb_llama_batch *b, void *stream);
  * rank's vocabulary rows). */
 int tcb_llama_batch_logits(tcb_llama_batch *b, float **logits);
 
+/* ---- Serving operators: paged K/V cache, attention over it, logits ----
+ *
+ * What a step of a batch of requests needs around the products: the plan of
+ * its pages, the append of its K/V rows, attention over the pages, and the
+ * penalties and masks on its logits.  TR keeps one contiguous cache per
+ * sequence (lib/layers.tr 126-215) and picks the first maximum
+ * (lib/layers.tr 712-770); these have no counterpart there.
+ *
+ * Every length and page number is read on the device, so a step can be
+ * captured once and replayed while the requests grow.  What the host cannot
+ * check is checked by the kernels: a length past max_len or past its table,
+ * a page or slot outside the pools, or more rows than max_rows leave
+ * TCB_ERR_BOUNDS in the device error word (tcb_device_error) and touch
+ * nothing outside the caller's arrays; the outputs of the request concerned
+ * are then unspecified.  Scratch is the context's: order calls on one context
+ * on one stream, and make one eager call of the largest shape before a
+ * stream capture. */
+
+/* A paged K/V cache: two pools of n_pages pages of `page` positions.  Element
+ * d of KV head h at position t of page g is at
+ *   g * page_stride + h * head_stride + t * pos_stride + d    (elements)
+ * in both pools, so [pages, heads, positions, hd] and [pages, positions,
+ * heads, hd] pools, and K and V interleaved in one array, are all views.
+ * dtype TCB_F16 or TCB_BF16; page 16, 32, 64, 128 or 256; head_dim 64 or
+ * 128; pool pointers on 16 bytes and strides in multiples of 8 elements. */
+typedef struct tcb_kv_pages {
+  void *k, *v;
+  int dtype, n_pages, page, n_kv_heads, head_dim;
+  long page_stride, head_stride, pos_stride;
+} tcb_kv_pages;
+
+/* The page plan of one step of B requests (at most TCB_PAGE_PLAN_MAX): from
+ * cached[b] positions in the cache and fresh[b] new ones,
+ *   need[b]  = ceil((cached[b] + fresh[b]) / page) - ceil(cached[b] / page)
+ *   tables[b][ceil(cached[b] / page) + j] = free_pages[n - 1 - (need[0] + .. + need[b-1] + j)],  j < need[b]
+ * (the free list is a stack of n = min(*n_free, free_cap) pages, taken from
+ * its end), and
+ *   row_start  [B + 1]  rows of request b are row_start[b] .. row_start[b+1]
+ *   kv_len     [B]      cached[b] + fresh[b]
+ *   slots, positions  [rows]  row i of request b: its position p = cached[b] + i
+ *              and its slot tables[b][p / page] * page + p % page; rows past
+ *              row_start[B] get -1
+ *   balance    [1]      n less need[0] + .. + need[b] of the last request b that is not
+ *              refused: the free pages left, or, below 0, how many the requests
+ *              refused before it lacked
+ *   taken      [1] or NULL  pages taken from the end of the free list
+ * A request is refused, with kv_len 0 and its rows' slots and positions -1,
+ * when a length of it is negative, its table (width entries, rows ldt apart)
+ * or the `rows` entries of slots do not hold it, or the free pages end before
+ * it has its share (as later ones that lack pages are then); it takes no
+ * page.  need is 0 for one that is refused on its lengths, rows or table.  The
+ * inputs are not changed (balance and taken are not the array n_free): the
+ * same call again gives the same. */
+#define TCB_PAGE_PLAN_MAX 8192
+int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached,
+                  const int *fresh, int *tables, int width, long ldt,
+                  const int *free_pages, int free_cap, const int *n_free,
+                  int rows, int *row_start, int *kv_len, int64_t *slots,
+                  int *positions, int *balance, int *taken, void *stream);
+
+/* Append T rows of K and V (row r, head h at k + r * ldx + h * head_dim, and
+ * v alike; F32, F16 or BF16) to the cache: row r goes to slot
+ * slots[r] = page number * page + position in the page, rounded once to the
+ * cache's type.  Rows with a negative slot are dropped.  Of two rows with one
+ * slot either may stay. */
+int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k,
+                  const void *v, int xdtype, long ldx, const int64_t *slots,
+                  void *stream);
+
+/* Attention of B requests over their pages, causal, with a sliding window
+ * and first positions that stay visible:
+ *   out[r, h] = sum_j p_j v[j] ,  p = softmax over the visible j of scale * q[r, h] . k[j]
+ * for row r = row_start[b] + i of request b, which stands at position
+ * p = kv_len[b] - (row_start[b+1] - row_start[b]) + i and sees
+ *   j <= p  with  j > p - window  or  j < sinks    (window < 0: every j <= p).
+ * Query head h reads KV head h / (H / n_kv_heads).  A row that sees nothing
+ * (p < 0, or window 0 without sinks) gives zeros; what the cache holds where
+ * a row does not look, NaN included, does not reach its result.
+ *   q, out     T rows of H heads of head_dim elements in the cache's type, ldq
+ *              and ldo elements apart; 16-byte aligned rows
+ *   row_start  device [B + 1], as tcb_page_plan writes it; rows of q outside
+ *              every request are left alone
+ *   kv_len     device [B], positions in the cache with this step's rows
+ *   tables     device [B][width] page numbers, rows ldt apart
+ *   max_rows   no request has more rows (1: a decode step)
+ *   max_len    no kv_len is larger
+ * Scores, softmax statistics and sums are in f32; the weights p_j are rounded
+ * to the cache's type for the tensor cores, as is the result. */
+int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H,
+                  const void *q, long ldq, void *out, long ldo,
+                  const int *row_start, const int *kv_len, const int *tables,
+                  int width, long ldt, int max_rows, int max_len, float scale,
+                  int window, int sinks, void *stream);
+
+/* A decode step's attention of B requests that share their first prefix_len
+ * positions, one row each (row b of q and out is request b):
+ *   out[b, h] = softmax over j < kv_len[b] of scale * q[b, h] . k[j], times v
+ * with positions j < prefix_len read from the pages prefix[j / page] (device,
+ * ceil(prefix_len / page) page numbers), once for all requests, and the
+ * others from tables[b][j / page] as in tcb_page_attn (entries of whole
+ * prefix pages are not read).  kv_len[b] may be below prefix_len; 0 gives
+ * zeros. */
+int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H,
+                    const void *q, long ldq, void *out, long ldo,
+                    const int *prefix, int prefix_len, const int *kv_len,
+                    const int *tables, int width, long ldt, int max_len,
+                    float scale, void *stream);
+
+/* Penalties, biases and masks on the logits of B sequences, and the pick.
+ * For token t of row b, in f32 and in this order, each step rounded once:
+ *   x = logits[b][t]
+ *   t among history[b][0 .. total_len[b]):  x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   n times among history[b][prompt_len[b] .. total_len[b]):  x -= frequency[b] * n,
+ *                                           and for n > 0  x -= presence[b]
+ *   t among bias_ids[b][0 .. n_bias):       x += bias[b][last such entry]
+ *   its bit of mask row mask_row[b] clear:  x = -inf
+ * out[b][t] = x, and token[b] is the first t of the largest x, NaN never
+ * picked; -1 when every x is -inf or NaN.  history holds token ids (prompt,
+ * then generated, as tcb_llama_buffers has them); ids outside [0, V) in
+ * history and bias_ids are unused entries.  Bit t % 32 of word t / 32 of a
+ * mask row allows token t; mask_row[b] < 0 masks nothing. */
+typedef struct tcb_logits_args {
+  int B, V;
+  const void *logits; int dtype; long ld;   /* F32, F16 or BF16, rows ld apart */
+  void *out; int odtype; long ldo;          /* may be logits itself, same type and stride */
+  int64_t *token;                           /* [B], or NULL */
+  /* [B][hist_width], rows ldh apart, and [B] lengths; NULL: no history.
+   * Lengths past hist_width count up to it; prompt_len NULL: no prompt. */
+  const int64_t *history; int hist_width; long ldh;
+  const int *prompt_len, *total_len;
+  const float *repetition, *frequency, *presence;  /* [B], NULL: 1, 0, 0 */
+  const int *bias_ids; const float *bias; int n_bias; long ldb;  /* [B][n_bias], NULL: none */
+  const uint32_t *mask; int n_masks; long ldm;  /* [n_masks][ceil(V / 32)], rows ldm apart; NULL: none */
+  const int *mask_row;                      /* [B]; NULL: row b of the mask */
+} tcb_logits_args;
+int tcb_logits_penalize(tcb_ctx *ctx, const tcb_logits_args *a, void *stream);
+
 /* Size of the device array that tcb_qgemm_act8_static works in. */
 #define TCB_STATIC_SCRATCH_BYTES (4u << 20)
 

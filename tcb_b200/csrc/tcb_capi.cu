@@ -61,7 +61,7 @@ int ensure_ws(tcb_ctx *ctx, size_t bytes) {
   return TCB_OK;
 }
 
-// grow one of the context's staging buffers (tcb_qgemm_host) to `bytes`
+// grow one of the context's staging buffers to `bytes`
 int ensure_buf(tcb_ctx *ctx, void **buf, size_t *cap, size_t bytes) {
   if (bytes <= *cap) return TCB_OK;
   if (*buf) {
@@ -254,6 +254,24 @@ int qgemm_tc_prologue(tcb_ctx *ctx, int wtype, int M, int N, int K, const void *
 }
 }  // namespace tcb
 
+namespace tcb {
+int ctx_fail(tcb_ctx *ctx, cudaError_t e) { return cuda_fail(ctx, e); }
+int ctx_bind(tcb_ctx *ctx) { return bind(ctx); }
+int ctx_ws(tcb_ctx *ctx, size_t bytes) {
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  return ensure_ws(ctx, bytes);
+}
+int ctx_tick(tcb_ctx *ctx, size_t bytes) {
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  if (bytes <= ctx->tick_cap) return TCB_OK;
+  int rc = ensure_buf(ctx, &ctx->tick, &ctx->tick_cap, bytes);
+  if (rc != TCB_OK) return rc;
+  TCB_CU(ctx, cudaMemset(ctx->tick, 0, ctx->tick_cap));
+  TCB_CU(ctx, cudaDeviceSynchronize());  // before a launch on any stream
+  return TCB_OK;
+}
+}  // namespace tcb
+
 namespace {
 using tcb::check_gemm_args;
 
@@ -331,7 +349,7 @@ int tcb_ctx_destroy(tcb_ctx *ctx) {
   if (!ctx) return TCB_OK;
   int rc = TCB_OK;
   if (cudaSetDevice(ctx->dev) != cudaSuccess) rc = TCB_ERR_CUDA;
-  for (void *p : {ctx->ws, (void *)ctx->derr, ctx->sk, ctx->hx, ctx->hc})
+  for (void *p : {ctx->ws, (void *)ctx->derr, ctx->sk, ctx->hx, ctx->hc, ctx->tick})
     if (p && cudaFree(p) != cudaSuccess) rc = TCB_ERR_CUDA;
   delete ctx;
   return rc;

@@ -1,6 +1,7 @@
 // tcb_ctx.h - the context behind the opaque tcb_ctx handle (internal).
 #pragma once
 
+#include <cuda_runtime.h>
 #include <stddef.h>
 
 #include <mutex>
@@ -17,6 +18,16 @@ struct tcb_ctx {
   size_t hx_cap = 0;
   void *hc = nullptr;   // tcb_qgemm_host: c of a caller whose c the GPU cannot reach
   size_t hc_cap = 0;
+  void *tick = nullptr;  // arrival counters and pick words of the logits kernel (zeroed; launches leave it zeroed)
+  size_t tick_cap = 0;
   std::mutex mu;
   char err[256] = {0};
 };
+
+// the context's helpers behind the C entry points (tcb_capi.cu)
+namespace tcb {
+int ctx_fail(tcb_ctx *ctx, cudaError_t e);        // record the error, TCB_ERR_CUDA
+int ctx_bind(tcb_ctx *ctx);                       // make the context's device current
+int ctx_ws(tcb_ctx *ctx, size_t bytes);           // at least `bytes` of scratch in ctx->ws
+int ctx_tick(tcb_ctx *ctx, size_t bytes);         // at least `bytes` of zeroed counters in ctx->tick
+}  // namespace tcb

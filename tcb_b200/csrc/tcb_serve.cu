@@ -1,0 +1,337 @@
+// tcb_serve.cu - the serving operators' C entry points (page plan, K/V
+// append, attention over the pages) with their argument checks, and the
+// kernels of the plan and the append.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/tcb.h"
+#include "tcb_common.cuh"
+#include "tcb_ctx.h"
+#include "tcb_page.h"
+
+namespace {
+
+bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
+int log2i(int v) { return v <= 1 ? 0 : 1 + log2i(v / 2); }
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// ------------------------------------------------------------ page plan
+
+constexpr int kPlanThreads = 256;
+
+struct PlanArgs {
+  int B, page, page_shift, width, free_cap, rows;
+  const int *cached, *fresh;
+  int *tables;
+  long ldt;
+  const int *free_pages, *n_free;
+  int *row_start, *kv_len;
+  int64_t *slots;
+  int *positions, *balance, *taken;
+};
+
+// exclusive sum over the CTA's threads, and the total
+__device__ long block_scan(long v, long *warp_sums, long &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  long before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; w++) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + x - v;
+}
+
+// the pages that a request lacks, -1 where its lengths, rows or table do not
+// hold it (row_end: one past its last row)
+__device__ __forceinline__ long pages_lacking(const PlanArgs &a, long cached, long fresh, long row_end) {
+  const long end = cached + fresh;
+  if (cached < 0 || fresh < 0 || row_end > a.rows || end > (long)a.width << a.page_shift || end > 0x7FFFFFFF) return -1;
+  return ((end + a.page - 1) >> a.page_shift) - ((cached + a.page - 1) >> a.page_shift);
+}
+
+// Every CTA scans all requests (two loads and two scans over at most
+// TCB_PAGE_PLAN_MAX requests) and keeps the row and page offsets in shared
+// memory, so the rows and table entries can be written by the whole grid in
+// one launch without waiting on one another.  Thread t holds the requests
+// t * items .. of its part; sums are 64-bit, so no length overflows them.
+__global__ void __launch_bounds__(kPlanThreads) k_page_plan(const PlanArgs a) {
+  extern __shared__ int sh[];
+  int *rs = sh;              // [B + 1] first row of each request
+  int *pg = sh + a.B + 1;    // [B] pages taken before it; -1: refused
+  __shared__ long sums[kPlanThreads / 32];
+  __shared__ int taken_s;
+  __shared__ long long asked_s;
+  const int tid = threadIdx.x;
+  const int items = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = tid * items, b1 = min(a.B, b0 + items);
+  const long n_free = min(max(*a.n_free, 0), a.free_cap);
+  if (tid == 0) taken_s = 0, asked_s = 0;
+
+  long sum = 0, total;
+  for (int b = b0; b < b1; b++) sum += max(a.fresh[b], 0);
+  long row = block_scan(sum, sums, total);
+  // the pages each request lacks, 0 where it does not fit its rows or table
+  const long r0 = row;
+  long lacks = 0;
+  for (int b = b0; b < b1; b++) {
+    const long f = a.fresh[b];
+    rs[b] = (int)min(row, (long)a.rows);
+    row += max(f, 0l);
+    lacks += max(pages_lacking(a, a.cached[b], f, row), 0l);
+  }
+  if (tid == 0) rs[a.B] = (int)min(total, (long)a.rows);
+  long page = block_scan(lacks, sums, total);
+  row = r0;
+  int taken = 0;       // by the last request that gets pages
+  long long asked = 0;  // up to the last one that is not refused
+  for (int b = b0; b < b1; b++) {
+    const long c = a.cached[b], f = a.fresh[b];
+    row += max(f, 0l);
+    const long need = pages_lacking(a, c, f, row);
+    const bool granted = need == 0 || (need > 0 && page + need <= n_free);
+    pg[b] = granted ? (int)min(page, n_free) : -1;
+    if (granted && need) taken = (int)(page + need);
+    if (granted) asked = page + need;
+    if (blockIdx.x == 0) {
+      a.row_start[b] = rs[b];
+      a.kv_len[b] = granted ? (int)(c + f) : 0;
+    }
+    page += max(need, 0l);
+  }
+  if (blockIdx.x == 0 && taken) atomicMax(&taken_s, taken);
+  if (blockIdx.x == 0 && asked) atomicMax(&asked_s, asked);
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) {
+    a.row_start[a.B] = rs[a.B];
+    *a.balance = (int)max(n_free - asked_s, -2147483647ll);
+    if (a.taken) *a.taken = taken_s;
+  }
+
+  // table entries: a warp per request
+  const int warps = gridDim.x * (kPlanThreads / 32), lane = tid & 31;
+  for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < a.B; b += warps) {
+    if (pg[b] < 0) continue;
+    const int c = a.cached[b];
+    const int have = (int)(((long)c + a.page - 1) >> a.page_shift);
+    const int need = (int)(((long)c + a.fresh[b] + a.page - 1) >> a.page_shift) - have;
+    for (int j = lane; j < need; j += 32) a.tables[b * a.ldt + have + j] = a.free_pages[n_free - 1 - pg[b] - j];
+  }
+  // rows: the request by bisection of the row offsets; a page that this call
+  // hands out is read from the free list, not from the table
+  for (long r = (long)blockIdx.x * kPlanThreads + tid; r < a.rows; r += (long)gridDim.x * kPlanThreads) {
+    int64_t slot = -1;
+    int pos = -1;
+    if (r < rs[a.B]) {
+      int lo = 0, hi = a.B;  // the last request whose first row is at or before r
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (rs[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      if (pg[lo] >= 0) {
+        const int c = a.cached[lo];
+        pos = c + (int)(r - rs[lo]);
+        const int have = (int)(((long)c + a.page - 1) >> a.page_shift), at = pos >> a.page_shift;
+        const int g = at < have ? a.tables[lo * a.ldt + at] : a.free_pages[n_free - 1 - pg[lo] - (at - have)];
+        if (g >= 0) slot = ((int64_t)g << a.page_shift) + (pos & (a.page - 1));
+      }
+    }
+    a.slots[r] = slot;
+    a.positions[r] = pos;
+  }
+}
+
+// ------------------------------------------------------------ append
+
+// 8 elements of one K or V row per thread: 16-byte loads where the rows are
+// 16-byte aligned (the cache always is), one rounding, one 16-byte store.
+// HBM-bound: T * KVH * hd * (x bytes + 2) * 2 bytes.
+template <int XT, bool VEC>
+__global__ void __launch_bounds__(256) k_kv_append(const tcb_kv_pages kv, int page_shift, int T, const void *k,
+                                                   const void *v, long ldx, const int64_t *slots, int *derr) {
+  const int per_head = kv.head_dim / 8, per_row = kv.n_kv_heads * per_head;
+  const long n = (long)T * per_row * 2;
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
+    const bool is_v = i >= n / 2;
+    const long j = is_v ? i - n / 2 : i;
+    const long r = j / per_row;
+    const int c = (int)(j - r * per_row), h = c / per_head, d = (c - h * per_head) * 8;
+    const int64_t slot = slots[r];
+    if (slot < 0) continue;
+    if (slot >= (int64_t)kv.n_pages << page_shift) {
+      if (c == 0) atomicExch(derr, TCB_ERR_BOUNDS);
+      continue;
+    }
+    const long x0 = r * ldx + (long)h * kv.head_dim + d;
+    const void *x = is_v ? v : k;
+    float f[8];
+    if constexpr (VEC) {
+      if constexpr (XT == TCB_F32) {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(x) + x0);
+        const float4 lo = p[0], hi = p[1];
+        f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(x) + x0);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint16_t b = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+          f[e] = XT == TCB_BF16 ? tcb::bf16_to_f32(b) : tcb::half_exact(b);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = tcb::load_act(x, x0 + e, XT);
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float a0 = f[2 * e], a1 = f[2 * e + 1];
+      o[e] = kv.dtype == TCB_BF16 ? tcb::f32_to_bf16(a0) | (uint32_t)tcb::f32_to_bf16(a1) << 16
+                                  : tcb::f32_to_f16(a0) | (uint32_t)tcb::f32_to_f16(a1) << 16;
+    }
+    uint16_t *dst = static_cast<uint16_t *>(is_v ? kv.v : kv.k) + (slot >> page_shift) * kv.page_stride +
+                    h * kv.head_stride + (slot & (kv.page - 1)) * kv.pos_stride + d;
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+int check_pages(const tcb_kv_pages *kv) {
+  if (!kv || !kv->k || !kv->v) return TCB_ERR_NULL;
+  if (kv->dtype != TCB_F16 && kv->dtype != TCB_BF16) return TCB_ERR_DTYPE;
+  if (!page_ok(kv->page) || kv->n_pages < 1 || kv->n_kv_heads < 1 || (kv->head_dim != 64 && kv->head_dim != 128))
+    return TCB_ERR_SHAPE;
+  if (kv->pos_stride < kv->head_dim || kv->head_stride < kv->head_dim || kv->page_stride < kv->head_dim)
+    return TCB_ERR_SHAPE;
+  if ((kv->pos_stride | kv->head_stride | kv->page_stride) % 8 || !aligned(kv->k, 16) || !aligned(kv->v, 16))
+    return TCB_ERR_ALIGN;
+  return TCB_OK;
+}
+
+// what tcb_page_attn and tcb_prefix_attn share
+int check_attn(const tcb_kv_pages *kv, int B, int T, int H, const void *q, long ldq, const void *out, long ldo,
+               const int *kv_len, const int *tables, int width, long ldt, int max_len, float scale) {
+  int rc = check_pages(kv);
+  if (rc != TCB_OK) return rc;
+  if (B < 0 || T < 0 || H < 1 || H % kv->n_kv_heads || B > 65535 || width < 0 || max_len < 0) return TCB_ERR_SHAPE;
+  if (!isfinite(scale)) return TCB_ERR_SHAPE;
+  if (B == 0 || T == 0) return TCB_OK;
+  if (ldq < (long)H * kv->head_dim || ldo < (long)H * kv->head_dim || (B > 1 && ldt < width)) return TCB_ERR_SHAPE;
+  if (!q || !out || !kv_len || (width > 0 && !tables)) return TCB_ERR_NULL;
+  if (!aligned(q, 16) || !aligned(out, 16) || ldq % 8 || ldo % 8) return TCB_ERR_ALIGN;
+  if (!aligned(kv_len, 4) || !aligned(tables, 4)) return TCB_ERR_ALIGN;
+  return TCB_OK;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+}  // namespace
+
+extern "C" {
+
+int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached, const int *fresh, int *tables, int width,
+                  long ldt, const int *free_pages, int free_cap, const int *n_free, int rows, int *row_start,
+                  int *kv_len, int64_t *slots, int *positions, int *balance, int *taken,
+                  void *stream) {
+  if (!ctx) return TCB_ERR_NULL;
+  if (B < 0 || !page_ok(page) || width < 0 || (B > 1 && ldt < width) || free_cap < 0 || rows < 0) return TCB_ERR_SHAPE;
+  if (B > TCB_PAGE_PLAN_MAX) return TCB_ERR_TOO_LARGE;
+  if (!row_start || !balance || !n_free || (B && (!cached || !fresh || !kv_len || (width && !tables))) ||
+      (free_cap && !free_pages) || (rows && (!slots || !positions)))
+    return TCB_ERR_NULL;
+  if (balance == n_free || taken == n_free) return TCB_ERR_UNSUPPORTED;  // the grid reads one while the other is written
+  for (const void *p : {(const void *)cached, (const void *)fresh, (const void *)tables, (const void *)free_pages,
+                        (const void *)n_free, (const void *)row_start, (const void *)kv_len, (const void *)positions,
+                        (const void *)balance, (const void *)taken})
+    if (!aligned(p, 4)) return TCB_ERR_ALIGN;
+  if (!aligned(slots, 8)) return TCB_ERR_ALIGN;
+  int rc = tcb::ctx_bind(ctx);
+  if (rc != TCB_OK) return rc;
+  PlanArgs a{B, page, log2i(page), width, free_cap, rows, cached, fresh, tables, ldt, free_pages, n_free,
+             row_start, kv_len, slots, positions, balance, taken};
+  const size_t smem = (2 * (size_t)B + 1) * sizeof(int);
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (2 * TCB_PAGE_PLAN_MAX + 1) * (int)sizeof(int));
+    if (e != cudaSuccess) return tcb::ctx_fail(ctx, e);
+  }
+  const long want = std::max<long>((rows + kPlanThreads - 1) / kPlanThreads, (B + kPlanThreads / 32 - 1) / (kPlanThreads / 32));
+  const int grid = (int)std::min<long>(std::max<long>(want, 1), 2 * ctx->sms);
+  k_page_plan<<<grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TCB_OK : tcb::ctx_fail(ctx, e);
+}
+
+int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k, const void *v, int xdtype, long ldx,
+                  const int64_t *slots, void *stream) {
+  if (!ctx) return TCB_ERR_NULL;
+  int rc = check_pages(kv);
+  if (rc != TCB_OK) return rc;
+  if (xdtype != TCB_F32 && xdtype != TCB_F16 && xdtype != TCB_BF16) return TCB_ERR_DTYPE;
+  if (T < 0) return TCB_ERR_SHAPE;
+  if (T == 0) return TCB_OK;
+  if (ldx < (long)kv->n_kv_heads * kv->head_dim) return TCB_ERR_SHAPE;
+  if (!k || !v || !slots) return TCB_ERR_NULL;
+  const size_t xe = xdtype == TCB_F32 ? 4 : 2;
+  if (!aligned(k, xe) || !aligned(v, xe) || !aligned(slots, 8)) return TCB_ERR_ALIGN;
+  if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
+  const bool vec = aligned(k, 16) && aligned(v, 16) && ldx * (long)xe % 16 == 0;
+  const long n = (long)T * kv->n_kv_heads * (kv->head_dim / 8) * 2;
+  const int grid = (int)std::min<long>((n + 255) / 256, 16l * ctx->sms);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sh = log2i(kv->page);
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(*kv, sh, T, k, v, ldx, slots, ctx->derr); };
+  if (xdtype == TCB_F32) vec ? go(k_kv_append<TCB_F32, true>) : go(k_kv_append<TCB_F32, false>);
+  else if (xdtype == TCB_F16) vec ? go(k_kv_append<TCB_F16, true>) : go(k_kv_append<TCB_F16, false>);
+  else vec ? go(k_kv_append<TCB_BF16, true>) : go(k_kv_append<TCB_BF16, false>);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TCB_OK : tcb::ctx_fail(ctx, e);
+}
+
+int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H, const void *q, long ldq, void *out,
+                  long ldo, const int *row_start, const int *kv_len, const int *tables, int width, long ldt,
+                  int max_rows, int max_len, float scale, int window, int sinks, void *stream) {
+  if (!ctx) return TCB_ERR_NULL;
+  int rc = check_attn(kv, B, T, H, q, ldq, out, ldo, kv_len, tables, width, ldt, max_len, scale);
+  if (rc != TCB_OK) return rc;
+  if (max_rows < 0 || sinks < 0) return TCB_ERR_SHAPE;
+  if (B == 0 || T == 0 || max_rows == 0) return TCB_OK;
+  if (!row_start) return TCB_ERR_NULL;
+  if (!aligned(row_start, 4)) return TCB_ERR_ALIGN;
+  if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
+  tcb::PageAttnArgs a{*kv, log2i(kv->page), B, T, H, q, ldq, out, ldo, row_start, kv_len, tables, width, ldt,
+                      nullptr, 0, std::min(max_rows, T), max_len, scale * kLog2e, window, sinks, ctx->derr};
+  return tcb::launch_page_attn(ctx, a, static_cast<cudaStream_t>(stream));
+}
+
+int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const void *q, long ldq, void *out, long ldo,
+                    const int *prefix, int prefix_len, const int *kv_len, const int *tables, int width, long ldt,
+                    int max_len, float scale, void *stream) {
+  if (!ctx) return TCB_ERR_NULL;
+  int rc = check_attn(kv, B, B, H, q, ldq, out, ldo, kv_len, tables, width, ldt, max_len, scale);
+  if (rc != TCB_OK) return rc;
+  if (prefix_len < 0) return TCB_ERR_SHAPE;
+  if (B == 0) return TCB_OK;
+  if (prefix_len && !prefix) return TCB_ERR_NULL;
+  if (!aligned(prefix, 4)) return TCB_ERR_ALIGN;
+  if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
+  tcb::PageAttnArgs a{*kv, log2i(kv->page), B, B, H, q, ldq, out, ldo, nullptr, kv_len, tables, width, ldt,
+                      prefix, prefix_len, 1, max_len, scale * kLog2e, -1, 0, ctx->derr};
+  return tcb::launch_page_attn(ctx, a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
