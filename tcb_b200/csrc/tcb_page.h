@@ -32,6 +32,8 @@ struct PageAttnArgs {
   int *derr;
 };
 
+// requests of one row (tcb_page_decode.cu)
+int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s);
 int launch_page_attn(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s);
 
 }  // namespace tcb

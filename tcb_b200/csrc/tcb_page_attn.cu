@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(128) k_page_attn_row(const PageAttnArgs a) {
 }  // namespace pa
 
 int launch_page_attn(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s) {
+  if (a.max_rows == 1 && a.row_start) return launch_page_decode(ctx, a, s);
   const dim3 grid((a.max_rows + 3) / 4, a.H, a.B);
   if (a.kv.head_dim == 64) pa::k_page_attn_row<64><<<grid, 128, 0, s>>>(a);
   else pa::k_page_attn_row<128><<<grid, 128, 0, s>>>(a);

@@ -1,0 +1,465 @@
+// tcb_page_decode.cu - attention over the paged cache for requests of one
+// row (a decode step; tcb_page_attn with max_rows 1).
+//
+// Mathematics: per (request, KV head) the G = H / KVH query heads that share
+// the head are the 8 or 16 columns of two products on the tensor cores,
+//   S^T = K Q^T   (16 positions x queries, per 16 positions)
+//   O^T += V^T P^T (head elements x queries)
+// with the running maximum m and sum l of the softmax per column, in powers of
+// two (scores times scale * log2 e).  m follows a column only when a score
+// passes it by more than kSlack (weights up to 2^kSlack, exact in f32 sums and
+// far inside f16's range), so the usual 16 positions cost no maximum across
+// lanes and no rescaling.
+//
+// Bound: the K/V bytes, each read once: at batch 64 about 3.6 GB.  Layout:
+// every fragment comes straight from global memory into registers, without
+// shared memory: the k slots of S^T are dealt so that a lane's A fragments of
+// K are 16-byte pieces of one position (lane (g, t): positions g and g + 8,
+// elements 32c + 8t ..; Q is read in the same order), and those of V^T are
+// 16-byte pieces of four positions (2t, 2t+1, 2t+8, 2t+9), paired by byte
+// permutes, with output row e of a lane group dealt to element 8g + e.  P^T
+// becomes a B fragment by one matrix transpose (movmatrix) per 8 positions.
+// A warp loads the next 16 positions' K as soon as it has formed S^T, and
+// their V as soon as it has added P V, so both stay in flight.
+//
+// Split: a cluster of up to 8 CTAs shares the positions of one (request, KV
+// head) in contiguous parts, 4 warps a CTA interleaved over 16-position
+// groups; the partial (m, l, O) are joined within the CTA through shared
+// memory and across the cluster through distributed shared memory, in a fixed
+// order, with no scratch in HBM and no second launch.  Where a few long
+// requests leave the GPU empty, several clusters share one: each rank leaves
+// its slice of the joined partial in scratch, and the rank that comes last
+// joins the slices.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "tcb_common.cuh"
+#include "tcb_page.h"
+
+namespace tcb {
+namespace pd {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kSlack = 8.f;
+constexpr uint32_t kAll = 0xFFFFFFFFu;
+
+template <int DT>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (DT == TCB_F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// CTAs per SM that leave a thread the registers it needs without spills (168
+// and 236 at head_dim 128).  At batch 64 with 3 CTAs: 554 us against 595 with
+// 4 and 128 spilling registers.
+template <int HD, int NT>
+constexpr int kCtas = (NT == 1 ? 4 : 3) - (HD == 128);
+
+// 16 bytes of the cache, read once: not kept in L1
+__device__ __forceinline__ uint4 ld_cache(const uint16_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// two weights rounded to the cache's type, and what they were rounded to
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float &a, float &b) {
+  uint32_t u;
+  if constexpr (DT == TCB_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    const float2 f = __half22float2(h);
+    a = f.x, b = f.y;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    u = *reinterpret_cast<const uint32_t *>(&h);
+    a = __uint_as_float(u << 16), b = __uint_as_float(u & 0xFFFF0000u);
+  }
+  return u;
+}
+
+// 2^(m - top) for a partial whose maximum is m; an empty one weighs 0
+__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+
+// where the partials of several clusters meet (parts > 1): element pairs
+// [unit][part][query][HD] and (m, l) [unit][part][rank][query], one counter per
+// (unit, rank); a unit is blockIdx.z * gridDim.y + blockIdx.y
+struct Join {
+  int parts, ranks;
+  float *o;
+  float2 *ml;
+  unsigned *arrived;  // zero before and after a launch
+};
+
+template <int DT, int HD, int NT>
+__global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const __grid_constant__ PageAttnArgs a,
+                                                                            const __grid_constant__ Join j) {
+  constexpr int Q = 8 * NT;  // query columns
+  constexpr int CK = HD / 32, CV = HD / 64;
+  __shared__ float so[kWarps][Q][HD];
+  __shared__ float sm[kWarps][Q], sl[kWarps][Q];
+  __shared__ float cm[Q], cl[Q];  // the CTA's
+  const int G = a.H / a.kv.n_kv_heads, tiles = (G + Q - 1) / Q;
+  const int kh = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * Q;  // first query head within the group
+  const int b = blockIdx.z, n_cta = gridDim.x;
+  const int n_rank = j.ranks, c = blockIdx.x % n_rank, part = blockIdx.x / n_rank;  // rank in the cluster; cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+  // the row of the request
+  int r = a.row_start[b];
+  const int rows = a.row_start[b + 1] - r;
+  bool bad = r < 0 || rows > 1;
+  const bool live = r >= 0 && r < a.T && rows >= 1;
+  int len = a.kv_len[b];
+  if (len < 0 || len > a.max_len || len > (long)a.width << a.page_shift) {
+    bad = true;
+    len = 0;
+  }
+  if (bad && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
+  if (!live) return;  // every CTA of the cluster leaves
+  // visible: [lo, len) and [0, first); 16-position groups [0, ns) and [w0, w1)
+  int lo = a.window < 0 ? 0 : (int)max(0l, (long)len - a.window);
+  int first = min(a.sinks, lo);
+  if (first == lo) lo = first = 0;
+  const int ns = (first + 15) >> 4, w0 = max(lo >> 4, ns), w1 = max((len + 15) >> 4, w0);
+  const int units = ns + w1 - w0;
+  const int u0 = (int)((long)units * blockIdx.x / n_cta), u1 = (int)((long)units * (blockIdx.x + 1) / n_cta);
+
+  // Q as the B operand: column g (and g + 8) is query head h0 + g
+  uint32_t qf[NT][2 * CK][2];
+  const long qrow = r * a.ldq + (long)(kh * G + h0) * HD;
+#pragma unroll
+  for (int x = 0; x < NT; x++) {
+    const bool ok = h0 + 8 * x + g < G;
+#pragma unroll
+    for (int e = 0; e < CK; e++) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (ok)
+        v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + qrow + (8 * x + g) * HD + 32 * e + 8 * t);
+      qf[x][2 * e][0] = v.x, qf[x][2 * e][1] = v.y, qf[x][2 * e + 1][0] = v.z, qf[x][2 * e + 1][1] = v.w;
+    }
+  }
+  float o[HD / 16][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int x = 0; x < NT; x++) {
+    m[x][0] = m[x][1] = -INFINITY;
+    l[x][0] = l[x][1] = 0.f;
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) o[d][x][0] = o[d][x][1] = o[d][x][2] = o[d][x][3] = 0.f;
+  }
+
+  const uint16_t *kp = static_cast<const uint16_t *>(a.kv.k) + kh * a.kv.head_stride + g * a.kv.pos_stride + 8 * t;
+  const uint16_t *vp = static_cast<const uint16_t *>(a.kv.v) + kh * a.kv.head_stride + 2 * t * a.kv.pos_stride + 8 * g;
+  const int *table = a.tables + b * a.ldt;
+  // lane i holds the page of the warp's group `base + i * kWarps` (-1: none such)
+  auto group_of = [&](int u) { return u < ns ? u : u - ns + w0; };
+  auto page_of = [&](int u) {
+    if (u >= u1) return 0;
+    const int pg = table[group_of(u) >> (a.page_shift - 4)];
+    return pg >= 0 && pg < a.kv.n_pages ? pg : -1;
+  };
+  const int base = u0 + warp, n_it = base < u1 ? (u1 - base + kWarps - 1) / kWarps : 0;
+  int pages = page_of(base + lane * kWarps), next_pages = 0;
+  if (n_it > 32) next_pages = page_of(base + (32 + lane) * kWarps);
+
+  uint4 kf[2 * CK], vf[4][CV];
+  // element offset of the group of iteration i, and whether its page is in the pools
+  bool page_bad = false;
+  auto locate = [&](int i, bool &ok) {
+    const int pg = __shfl_sync(kAll, pages, i & 31);
+    const int pos = group_of(base + i * kWarps) << 4;
+    ok = pg >= 0;
+    return (ok ? pg : 0) * a.kv.page_stride + (pos & (a.kv.page - 1)) * a.kv.pos_stride;
+  };
+  auto load_k = [&](long off) {
+#pragma unroll
+    for (int e = 0; e < CK; e++) {
+      kf[e] = ld_cache(kp + off + 32 * e);
+      kf[CK + e] = ld_cache(kp + off + 8 * a.kv.pos_stride + 32 * e);
+    }
+  };
+  auto load_v = [&](long off) {
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+      for (int e = 0; e < CV; e++)
+        vf[x][e] = ld_cache(vp + off + ((x & 1) + 8 * (x >> 1)) * a.kv.pos_stride + 64 * e);
+  };
+  bool ok = true;
+  if (n_it > 0) {
+    const long off = locate(0, ok);
+    load_k(off);
+    load_v(off);
+  }
+  for (int i = 0; i < n_it; i++) {
+    const bool here = ok;
+    const int key0 = group_of(base + i * kWarps) << 4;
+    float s[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+      s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < CK; e++) {
+        mma<DT>(s[x], kf[e].x, kf[CK + e].x, kf[e].y, kf[CK + e].y, qf[x][2 * e][0], qf[x][2 * e][1]);
+        mma<DT>(s[x], kf[e].z, kf[CK + e].z, kf[e].w, kf[CK + e].w, qf[x][2 * e + 1][0], qf[x][2 * e + 1][1]);
+      }
+    }
+    // the next group's K
+    long off = 0;
+    if (i + 1 < n_it) {
+      if (((i + 1) & 31) == 0) {
+        pages = next_pages;
+        next_pages = page_of(base + (i + 33 + lane) * kWarps);
+      }
+      off = locate(i + 1, ok);
+      load_k(off);
+    }
+    const bool edge = !here || key0 + 16 > len || (key0 < lo && key0 + 16 > first);
+    auto sees = [&](int key) { return here && key < len && (key >= lo || key < first); };
+    bool up = false;
+#pragma unroll
+    for (int x = 0; x < NT; x++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s[x][e] *= a.scale_log2;
+        if (edge && !sees(key0 + g + 8 * (e >> 1))) s[x][e] = -INFINITY;
+        up |= s[x][e] > m[x][e & 1] + kSlack;
+      }
+    if (__any_sync(kAll, up)) {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float top = fmaxf(s[x][e], s[x][2 + e]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, w));
+          top = fmaxf(top, m[x][e]);
+          const float keep = join_weight(m[x][e], top);
+          m[x][e] = top;
+          l[x][e] *= keep;
+#pragma unroll
+          for (int d = 0; d < HD / 16; d++) o[d][x][e] *= keep, o[d][x][2 + e] *= keep;
+        }
+    }
+    uint32_t pf[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+      const float m0 = m[x][0] == -INFINITY ? 0.f : m[x][0], m1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float p0 = exp2_fast(s[x][2 * e] - m0), p1 = exp2_fast(s[x][2 * e + 1] - m1);
+        pf[x][e] = transpose8x8(pack2<DT>(p0, p1));
+        l[x][0] += p0;
+        l[x][1] += p1;
+      }
+    }
+    if (edge) {  // what no query sees is not multiplied by 0 but left out
+      page_bad |= !here;
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+        if (!sees(key0 + 2 * t + (x & 1) + 8 * (x >> 1)))
+#pragma unroll
+          for (int e = 0; e < CV; e++) vf[x][e] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < CV; e++) {
+      const uint32_t *v0 = &vf[0][e].x, *v1 = &vf[1][e].x, *v2 = &vf[2][e].x, *v3 = &vf[3][e].x;
+#pragma unroll
+      for (int d = 0; d < 4; d++) {
+        const uint32_t a0 = __byte_perm(v0[d], v1[d], 0x5410), a1 = __byte_perm(v0[d], v1[d], 0x7632);
+        const uint32_t a2 = __byte_perm(v2[d], v3[d], 0x5410), a3 = __byte_perm(v2[d], v3[d], 0x7632);
+#pragma unroll
+        for (int x = 0; x < NT; x++) mma<DT>(o[4 * e + d][x], a0, a1, a2, a3, pf[x][0], pf[x][1]);
+      }
+    }
+    if (i + 1 < n_it) load_v(off);
+  }
+  if (page_bad && lane == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
+
+  // the CTA's partial: o[4e + d] of lane (g, t) holds, for queries 2t and 2t + 1,
+  // elements 64e + 8g + 2d and the next
+#pragma unroll
+  for (int x = 0; x < NT; x++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[x][e] += __shfl_xor_sync(kAll, l[x][e], w);
+      const int q = 8 * x + 2 * t + e;
+      if (g == 0) sm[warp][q] = m[x][e], sl[warp][q] = l[x][e];
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++)
+        *reinterpret_cast<float2 *>(&so[warp][q][64 * (d >> 2) + 8 * g + 2 * (d & 3)]) =
+            make_float2(o[d][x][e], o[d][x][2 + e]);
+    }
+  __syncthreads();
+  const int per_row = HD / 2;  // pairs of elements
+  for (int i = threadIdx.x; i < Q * per_row; i += kThreads) {
+    const int q = i / per_row, d = 2 * (i - q * per_row);
+    float top = sm[0][q];
+#pragma unroll
+    for (int w = 1; w < kWarps; w++) top = fmaxf(top, sm[w][q]);
+    float2 acc = make_float2(0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const float f = join_weight(sm[w][q], top);
+      const float2 v = *reinterpret_cast<const float2 *>(&so[w][q][d]);
+      acc.x += f * v.x, acc.y += f * v.y;
+      sum += f * sl[w][q];
+    }
+    *reinterpret_cast<float2 *>(&so[0][q][d]) = acc;  // read by this thread alone
+    if (d == 0) cm[q] = top, cl[q] = sum;
+  }
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (n_rank > 1) cluster.sync();
+  else __syncthreads();
+  // this rank's slice of the outputs, over the cluster's partials in rank order
+  const int live_q = min(Q, G - h0), all = live_q * per_row;
+  uint16_t *out = static_cast<uint16_t *>(a.out) + r * a.ldo + (long)(kh * G + h0) * HD;
+  auto store = [&](int q, int d, float2 acc, float sum) {
+    float x = sum == 0.f ? 0.f : __fdiv_rn(acc.x, sum), y = sum == 0.f ? 0.f : __fdiv_rn(acc.y, sum);
+    *reinterpret_cast<uint32_t *>(out + (long)q * HD + d) = pack2<DT>(x, y);
+  };
+  const long unit = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  auto part_o = [&](int w, int q, int d) {
+    return reinterpret_cast<float2 *>(j.o + ((unit * j.parts + w) * Q + q) * HD + d);
+  };
+  auto part_ml = [&](int w, int q) { return j.ml + ((unit * j.parts + w) * n_rank + c) * Q + q; };
+  for (int i = c * kThreads + threadIdx.x; i < all; i += n_rank * kThreads) {
+    const int q = i / per_row, d = 2 * (i - q * per_row);
+    float top = -INFINITY, sum = 0.f;
+    float2 acc = make_float2(0.f, 0.f);
+    for (int w = 0; w < n_rank; w++) top = fmaxf(top, *cluster.map_shared_rank(&cm[q], w));
+    for (int w = 0; w < n_rank; w++) {
+      const float f = join_weight(*cluster.map_shared_rank(&cm[q], w), top);
+      const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&so[0][q][d], w));
+      acc.x += f * v.x, acc.y += f * v.y;
+      sum += f * *cluster.map_shared_rank(&cl[q], w);
+    }
+    if (j.parts == 1) {
+      store(q, d, acc, sum);
+    } else {
+      __stcg(part_o(part, q, d), acc);
+      __stcg(part_ml(part, q), make_float2(top, sum));  // the same value from every thread of the query
+    }
+  }
+  if (n_rank > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+  if (j.parts == 1) return;
+  // the last of the clusters' ranks c joins their slices, in cluster order
+  __threadfence();
+  __syncthreads();
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    unsigned *n = j.arrived + unit * n_rank + c;
+    last = atomicAdd(n, 1u) == (unsigned)j.parts - 1;
+    if (last) *n = 0;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = c * kThreads + threadIdx.x; i < all; i += n_rank * kThreads) {
+    const int q = i / per_row, d = 2 * (i - q * per_row);
+    float top = -INFINITY, sum = 0.f;
+    float2 acc = make_float2(0.f, 0.f);
+    for (int w = 0; w < j.parts; w++) top = fmaxf(top, __ldcg(part_ml(w, q)).x);
+    for (int w = 0; w < j.parts; w++) {
+      const float2 ml = __ldcg(part_ml(w, q)), v = __ldcg(part_o(w, q, d));
+      const float f = join_weight(ml.x, top);
+      acc.x += f * v.x, acc.y += f * v.y;
+      sum += f * ml.y;
+    }
+    store(q, d, acc, sum);
+  }
+}
+
+template <int DT, int HD, int NT>
+int launch(tcb_ctx *ctx, const PageAttnArgs &a, int units, int split, cudaStream_t s) {
+  constexpr int Q = 8 * NT;
+  Join j = {};
+  j.ranks = std::min(split, 8);
+  j.parts = split / j.ranks;
+  if (j.parts > 1) {
+    const size_t n = (size_t)units * j.parts, o = n * Q * HD * sizeof(float);
+    int rc = ctx_ws(ctx, o + n * j.ranks * Q * sizeof(float2));
+    if (rc != TCB_OK || (rc = ctx_tick(ctx, (size_t)units * j.ranks * sizeof(unsigned))) != TCB_OK) return rc;
+    j.o = static_cast<float *>(ctx->ws);
+    j.ml = reinterpret_cast<float2 *>(static_cast<char *>(ctx->ws) + o);
+    j.arrived = static_cast<unsigned *>(ctx->tick);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(split, units / a.B, a.B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = j.ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_page_decode<DT, HD, NT>, a, j);
+  return e == cudaSuccess ? TCB_OK : ctx_fail(ctx, e);
+}
+
+}  // namespace pd
+
+int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s) {
+  const int G = a.H / a.kv.n_kv_heads, nt = G <= 8 ? 1 : 2;
+  const long seen = a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
+  const long groups = (seen + 15) / 16;  // of 16 positions, in the longest request
+  const long units = (long)a.B * a.kv.n_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
+  // CTAs per unit, doubled
+  //  - while one wave of CTAs holds them (about 4 a SM) and a warp keeps 2 groups: one
+  //    sequence with 1024 positions in sight takes 8.2 us with 8, 9.4 with 4;
+  //    one of 32768 with one KV head 17.1 with 128, 64.9 with 8
+  //  - up to a cluster, while there are fewer than about 4 waves and a warp keeps
+  //    128 KB of K and V, to even out ragged lengths: 64 sequences of up to
+  //    32768, 8 KV heads: 554 us with 4 (2048 CTAs), 574 with 8, 645 with 2
+  int split = 1;
+  while (split < 128) {
+    const long per_warp = groups / (2 * split * pd::kWarps), ctas = units * split;
+    if (2 * ctas <= 4 * 148 && per_warp >= 2) split *= 2;
+    else if (split < 8 && ctas < 12 * 148 && per_warp * 16 * a.kv.head_dim * 4 >= 128 << 10) split *= 2;
+    else break;
+  }
+  const bool h = a.kv.dtype == TCB_F16, wide = a.kv.head_dim == 128;
+  const int n = (int)units;
+  if (nt == 1) {
+    if (wide) return h ? pd::launch<TCB_F16, 128, 1>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 128, 1>(ctx, a, n, split, s);
+    return h ? pd::launch<TCB_F16, 64, 1>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 64, 1>(ctx, a, n, split, s);
+  }
+  if (wide) return h ? pd::launch<TCB_F16, 128, 2>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 128, 2>(ctx, a, n, split, s);
+  return h ? pd::launch<TCB_F16, 64, 2>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 64, 2>(ctx, a, n, split, s);
+}
+
+}  // namespace tcb
