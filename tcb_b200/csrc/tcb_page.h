@@ -32,8 +32,33 @@ struct PageAttnArgs {
   int *derr;
 };
 
-// requests of one row (tcb_page_decode.cu)
-int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s);
-int launch_page_attn(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s);
+// Requests of many rows, and the shared prefix of a batch (a.prefix set: all
+// T rows against its positions): tcb_page_rows.cu.  With more than one CTA
+// along the positions, and for a prefix, the kernel leaves partial results
+// in scratch: o[split][T * H][head_dim] and, o_bytes on, (maximum, sum)
+// pairs [split][T * H]; a prefix's are joined by the kernel of its suffixes.
+struct RowsPlan {
+  int tiles, split;
+  bool partial;
+  size_t o_bytes, bytes;
+};
+RowsPlan page_rows_plan(const PageAttnArgs &a);
+int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, void *scratch, cudaStream_t s);
+
+// Requests of one row (tcb_page_decode.cu).  With a.prefix set: the positions
+// from a.prefix_len on, joined with `parts` partial results as above.
+struct DecodePlan {
+  int nt, units, split;
+  size_t o_bytes, bytes;  // scratch of the join across clusters
+  size_t counters;        // bytes of zeroed counters
+};
+struct PrefixPartials {
+  int parts;
+  const float *o;
+  const float2 *ml;
+};
+DecodePlan page_decode_plan(const PageAttnArgs &a);
+int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, const DecodePlan &pl, void *scratch, const PrefixPartials &x,
+                       cudaStream_t s);
 
 }  // namespace tcb

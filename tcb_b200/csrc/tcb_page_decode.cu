@@ -123,7 +123,8 @@ struct Join {
 
 template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const __grid_constant__ PageAttnArgs a,
-                                                                            const __grid_constant__ Join j) {
+                                                                            const __grid_constant__ Join j,
+                                                                            const __grid_constant__ PrefixPartials x) {
   constexpr int Q = 8 * NT;  // query columns
   constexpr int CK = HD / 32, CV = HD / 64;
   __shared__ float so[kWarps][Q][HD];
@@ -136,8 +137,11 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   // the row of the request
-  int r = a.row_start[b];
-  const int rows = a.row_start[b + 1] - r;
+  int r = b, rows = 1;
+  if (a.row_start) {
+    r = a.row_start[b];
+    rows = a.row_start[b + 1] - r;
+  }
   bool bad = r < 0 || rows > 1;
   const bool live = r >= 0 && r < a.T && rows >= 1;
   int len = a.kv_len[b];
@@ -148,10 +152,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   if (bad && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
   if (!live) return;  // every CTA of the cluster leaves
   // visible: [lo, len) and [0, first); 16-position groups [0, ns) and [w0, w1)
-  int lo = a.window < 0 ? 0 : (int)max(0l, (long)len - a.window);
+  int lo = a.window < 0 ? min(a.prefix_len, len) : (int)max(0l, (long)len - a.window);
   int first = min(a.sinks, lo);
-  if (first == lo) lo = first = 0;
-  const int ns = (first + 15) >> 4, w0 = max(lo >> 4, ns), w1 = max((len + 15) >> 4, w0);
+  if (first == lo && first > 0) lo = first = 0;
+  const int ns = (first + 15) >> 4, w0 = max(lo >> 4, ns), w1 = lo < len ? max((len + 15) >> 4, w0) : w0;
   const int units = ns + w1 - w0;
   const int u0 = (int)((long)units * blockIdx.x / n_cta), u1 = (int)((long)units * (blockIdx.x + 1) / n_cta);
 
@@ -347,9 +351,22 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   // this rank's slice of the outputs, over the cluster's partials in rank order
   const int live_q = min(Q, G - h0), all = live_q * per_row;
   uint16_t *out = static_cast<uint16_t *>(a.out) + r * a.ldo + (long)(kh * G + h0) * HD;
-  auto store = [&](int q, int d, float2 acc, float sum) {
-    float x = sum == 0.f ? 0.f : __fdiv_rn(acc.x, sum), y = sum == 0.f ? 0.f : __fdiv_rn(acc.y, sum);
-    *reinterpret_cast<uint32_t *>(out + (long)q * HD + d) = pack2<DT>(x, y);
+  auto store = [&](int q, int d, float2 acc, float top, float sum) {
+    if (x.parts) {  // the prefix, in the order of its parts
+      const long row = (long)r * a.H + kh * G + h0 + q, all_rows = (long)a.T * a.H;
+      float joint = top;
+      for (int w = 0; w < x.parts; w++) joint = fmaxf(joint, __ldcg(x.ml + w * all_rows + row).x);
+      const float f = join_weight(top, joint);
+      acc.x *= f, acc.y *= f, sum *= f;
+      for (int w = 0; w < x.parts; w++) {
+        const float2 ml = __ldcg(x.ml + w * all_rows + row);
+        const float2 v = __ldcg(reinterpret_cast<const float2 *>(x.o + (w * all_rows + row) * HD + d));
+        const float g = join_weight(ml.x, joint);
+        acc.x += g * v.x, acc.y += g * v.y, sum += g * ml.y;
+      }
+    }
+    float v0 = sum == 0.f ? 0.f : __fdiv_rn(acc.x, sum), v1 = sum == 0.f ? 0.f : __fdiv_rn(acc.y, sum);
+    *reinterpret_cast<uint32_t *>(out + (long)q * HD + d) = pack2<DT>(v0, v1);
   };
   const long unit = (long)blockIdx.z * gridDim.y + blockIdx.y;
   auto part_o = [&](int w, int q, int d) {
@@ -368,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
       sum += f * *cluster.map_shared_rank(&cl[q], w);
     }
     if (j.parts == 1) {
-      store(q, d, acc, sum);
+      store(q, d, acc, top, sum);
     } else {
       __stcg(part_o(part, q, d), acc);
       __stcg(part_ml(part, q), make_float2(top, sum));  // the same value from every thread of the query
@@ -399,26 +416,14 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
       acc.x += f * v.x, acc.y += f * v.y;
       sum += f * ml.y;
     }
-    store(q, d, acc, sum);
+    store(q, d, acc, top, sum);
   }
 }
 
 template <int DT, int HD, int NT>
-int launch(tcb_ctx *ctx, const PageAttnArgs &a, int units, int split, cudaStream_t s) {
-  constexpr int Q = 8 * NT;
-  Join j = {};
-  j.ranks = std::min(split, 8);
-  j.parts = split / j.ranks;
-  if (j.parts > 1) {
-    const size_t n = (size_t)units * j.parts, o = n * Q * HD * sizeof(float);
-    int rc = ctx_ws(ctx, o + n * j.ranks * Q * sizeof(float2));
-    if (rc != TCB_OK || (rc = ctx_tick(ctx, (size_t)units * j.ranks * sizeof(unsigned))) != TCB_OK) return rc;
-    j.o = static_cast<float *>(ctx->ws);
-    j.ml = reinterpret_cast<float2 *>(static_cast<char *>(ctx->ws) + o);
-    j.arrived = static_cast<unsigned *>(ctx->tick);
-  }
+cudaError_t launch(const PageAttnArgs &a, const DecodePlan &pl, const Join &j, const PrefixPartials &x, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(split, units / a.B, a.B);
+  cfg.gridDim = dim3(pl.split, pl.units / a.B, a.B);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -427,17 +432,21 @@ int launch(tcb_ctx *ctx, const PageAttnArgs &a, int units, int split, cudaStream
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_page_decode<DT, HD, NT>, a, j);
-  return e == cudaSuccess ? TCB_OK : ctx_fail(ctx, e);
+  return cudaLaunchKernelEx(&cfg, k_page_decode<DT, HD, NT>, a, j, x);
 }
 
 }  // namespace pd
 
-int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s) {
-  const int G = a.H / a.kv.n_kv_heads, nt = G <= 8 ? 1 : 2;
-  const long seen = a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
+DecodePlan page_decode_plan(const PageAttnArgs &a) {
+  DecodePlan pl{};
+  const int G = a.H / a.kv.n_kv_heads;
+  pl.nt = G <= 8 ? 1 : 2;
+  const int q = 8 * pl.nt;
+  long seen = a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
+  if (a.prefix) seen = std::max(0, a.max_len - a.prefix_len) + 16;
   const long groups = (seen + 15) / 16;  // of 16 positions, in the longest request
-  const long units = (long)a.B * a.kv.n_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
+  const long units = (long)a.B * a.kv.n_kv_heads * ((G + q - 1) / q);
+  pl.units = (int)units;
   // CTAs per unit, doubled
   //  - while one wave of CTAs holds them (about 4 a SM) and a warp keeps 2 groups: one
   //    sequence with 1024 positions in sight takes 8.2 us with 8, 9.4 with 4;
@@ -452,14 +461,38 @@ int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, cudaStream_t s) {
     else if (split < 8 && ctas < 12 * 148 && per_warp * 16 * a.kv.head_dim * 4 >= 128 << 10) split *= 2;
     else break;
   }
-  const bool h = a.kv.dtype == TCB_F16, wide = a.kv.head_dim == 128;
-  const int n = (int)units;
-  if (nt == 1) {
-    if (wide) return h ? pd::launch<TCB_F16, 128, 1>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 128, 1>(ctx, a, n, split, s);
-    return h ? pd::launch<TCB_F16, 64, 1>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 64, 1>(ctx, a, n, split, s);
+  pl.split = split;
+  if (split > 8) {
+    const size_t n = (size_t)units * (split / 8);
+    pl.o_bytes = n * q * a.kv.head_dim * sizeof(float);
+    pl.bytes = pl.o_bytes + n * 8 * q * sizeof(float2);
+    pl.counters = (size_t)units * 8 * sizeof(unsigned);
   }
-  if (wide) return h ? pd::launch<TCB_F16, 128, 2>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 128, 2>(ctx, a, n, split, s);
-  return h ? pd::launch<TCB_F16, 64, 2>(ctx, a, n, split, s) : pd::launch<TCB_BF16, 64, 2>(ctx, a, n, split, s);
+  return pl;
+}
+
+int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, const DecodePlan &pl, void *scratch, const PrefixPartials &x,
+                       cudaStream_t s) {
+  pd::Join j{};
+  j.ranks = std::min(pl.split, 8);
+  j.parts = pl.split / j.ranks;
+  if (j.parts > 1) {
+    const int rc = ctx_tick(ctx, pl.counters);
+    if (rc != TCB_OK) return rc;
+    j.o = static_cast<float *>(scratch);
+    j.ml = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + pl.o_bytes);
+    j.arrived = static_cast<unsigned *>(ctx->tick);
+  }
+  const bool h = a.kv.dtype == TCB_F16, wide = a.kv.head_dim == 128;
+  cudaError_t e;
+  if (pl.nt == 1) {
+    if (wide) e = h ? pd::launch<TCB_F16, 128, 1>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 1>(a, pl, j, x, s);
+    else e = h ? pd::launch<TCB_F16, 64, 1>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 1>(a, pl, j, x, s);
+  } else {
+    if (wide) e = h ? pd::launch<TCB_F16, 128, 2>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 2>(a, pl, j, x, s);
+    else e = h ? pd::launch<TCB_F16, 64, 2>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 2>(a, pl, j, x, s);
+  }
+  return e == cudaSuccess ? TCB_OK : ctx_fail(ctx, e);
 }
 
 }  // namespace tcb

@@ -315,7 +315,15 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H, con
   if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
   tcb::PageAttnArgs a{*kv, log2i(kv->page), B, T, H, q, ldq, out, ldo, row_start, kv_len, tables, width, ldt,
                       nullptr, 0, std::min(max_rows, T), max_len, scale * kLog2e, window, sinks, ctx->derr};
-  return tcb::launch_page_attn(ctx, a, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (max_rows == 1) {
+    const tcb::DecodePlan pl = tcb::page_decode_plan(a);
+    if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
+    return tcb::launch_page_decode(ctx, a, pl, ctx->ws, {}, s);
+  }
+  const tcb::RowsPlan pl = tcb::page_rows_plan(a);
+  if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
+  return tcb::launch_page_rows(ctx, a, pl, ctx->ws, s);
 }
 
 int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const void *q, long ldq, void *out, long ldo,
@@ -330,8 +338,20 @@ int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const vo
   if (!aligned(prefix, 4)) return TCB_ERR_ALIGN;
   if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
   tcb::PageAttnArgs a{*kv, log2i(kv->page), B, B, H, q, ldq, out, ldo, nullptr, kv_len, tables, width, ldt,
-                      prefix, prefix_len, 1, max_len, scale * kLog2e, -1, 0, ctx->derr};
-  return tcb::launch_page_attn(ctx, a, static_cast<cudaStream_t>(stream));
+                      prefix_len ? prefix : nullptr, prefix_len, 1, max_len, scale * kLog2e, -1, 0, ctx->derr};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const tcb::DecodePlan dp = tcb::page_decode_plan(a);
+  tcb::RowsPlan rp{};
+  if (prefix_len) rp = tcb::page_rows_plan(a);
+  const size_t at = (rp.bytes + 255) / 256 * 256;
+  if ((rc = tcb::ctx_ws(ctx, at + dp.bytes)) != TCB_OK) return rc;
+  char *ws = static_cast<char *>(ctx->ws);
+  tcb::PrefixPartials x{};
+  if (prefix_len) {
+    if ((rc = tcb::launch_page_rows(ctx, a, rp, ws, s)) != TCB_OK) return rc;
+    x = {rp.split, reinterpret_cast<const float *>(ws), reinterpret_cast<const float2 *>(ws + rp.o_bytes)};
+  }
+  return tcb::launch_page_decode(ctx, a, dp, ws + at, x, s);
 }
 
 }  // extern "C"
