@@ -17,17 +17,17 @@
 //
 //   warp 0      K and V tiles by TMA from the pages (128-byte swizzle; one box
 //               per page and 64 elements, one lane each), 2 stages of each
-//   warp 1      tensor-memory allocation, MMA issue (one thread)
+//   warp 1      tensor-memory allocation, MMA issue
 //   warps 2, 3  V tiles at the edge of some row's sight (see below)
 //   warps 4-7, 8-11  softmax of tile 0 and 1: thread = row = lane of tensor
 //               memory; they also load Q and write the result
 //
 // Masked positions: a row's weight there is 0, but 0 times a non-finite V is
 // not.  Tiles that some row of the CTA sees only in part are gone through by
-// warps 2 and 3 before the product: positions past the last row's are zeroed
-// (they may be unwritten memory), and non-finite V elements are set to 0 and
-// remembered; if any were found, the rows that do see them add them at the
-// end.  Tiles in full sight of every row need nothing.
+// warps 2 and 3 before the product: positions that no row sees are zeroed (they may
+// be unwritten memory), and non-finite V elements of those that some rows see
+// are set to 0 and noted; if any were found, the rows that do see them add them
+// at the end.  Tiles in full sight of every row need nothing.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -150,6 +150,25 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase, volatile int
   atomicExch(err, TCB_ERR_TIMEOUT);
   return false;
 }
+// A barrier that other warps arrive on: a suspended try_wait wakes late from
+// those (about 700 cycles), so it is polled (with or without the sleep is the
+// same time).
+__device__ __forceinline__ bool wait_polled(uint64_t *bar, uint32_t phase, volatile int *stop, int *err) {
+  for (uint32_t i = 0; i < 1u << 26; i++) {
+    if (mv::mbar_test_wait(bar, phase)) return true;
+    if (*stop) return false;
+    __nanosleep(32);
+  }
+  *stop = 1;
+  atomicExch(err, TCB_ERR_TIMEOUT);
+  return false;
+}
+// one thread of a converged warp
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 // the same after another role has given up (copies and products in flight)
 __device__ __forceinline__ void drain(uint64_t *bar, uint32_t phase) {
   for (uint32_t i = 0; i < 1u << 20; i++)
@@ -178,9 +197,40 @@ __device__ __forceinline__ bool nonfinite2(uint32_t u) {
   return (u & e) == e || (u >> 16 & e) == e;
 }
 
+// pairs of f32 in one register pair: one instruction for two lanes
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// the larger of three, NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// bits 0 .. n-1
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? kAll : (1u << n) - 1u; }
+
 struct Bars {
   uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vready[kStages], vempty[kStages];
-  uint64_t qready, sfull[kTiles], pready[kTiles], odone[kTiles];
+  uint64_t qready, sfull[kTiles], phalf[kTiles], pready[kTiles], odone[kTiles];
   uint64_t checked, drained;
 };
 
@@ -203,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   __shared__ volatile int stop;
   __shared__ int dirty;
   const PageAttnArgs &a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(kAll, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the warp's number in a uniform register
   const int part = blockIdx.x % p.split, tile = p.tiles - 1 - (int)(blockIdx.x / p.split);  // the longest first
   const int kh = blockIdx.y, b = blockIdx.z;
 
@@ -240,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     mbar_init(&bar.drained, 1);
     for (int i = 0; i < kTiles; i++) {
       mbar_init(bar.sfull + i, 1);
+      mbar_init(bar.phalf + i, kRows);
       mbar_init(bar.pready + i, kRows);
       mbar_init(bar.odone + i, 1);
     }
@@ -271,10 +322,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       first = min(a.sinks, lo);
       if (first == lo) lo = first = 0;
     }
-    atomicMin(&hi_min, hi), atomicMax(&hi_max, hi);
-    if (hi > 0) {
-      atomicMin(&lo_min, lo), atomicMax(&lo_max, lo);
-      atomicMin(&first_min, first), atomicMax(&first_max, first);
+  }
+  if (qt >= 0) {
+    // rows that see something bound the tiles; every row bounds the full sight
+    const int far = 0x7FFFFFFF;
+    const int v[6] = {__reduce_min_sync(kAll, live ? hi : far), __reduce_max_sync(kAll, hi),
+                      __reduce_min_sync(kAll, hi > 0 ? lo : far), __reduce_max_sync(kAll, lo),
+                      __reduce_min_sync(kAll, hi > 0 ? first : far), __reduce_max_sync(kAll, first)};
+    if (lane == 0) {
+      atomicMin(&hi_min, v[0]), atomicMax(&hi_max, v[1]), atomicMin(&lo_min, v[2]);
+      atomicMax(&lo_max, v[3]), atomicMin(&first_min, v[4]), atomicMax(&first_max, v[5]);
     }
   }
   __syncthreads();
@@ -293,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
       // K and V: lane = (box of the tile, 64 elements)
       const int boxes = kKeys / p.box, at = lane / (HD / 64), half = lane % (HD / 64);
@@ -335,92 +392,117 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         for (int t = nv - 1; t >= max(0, nv - kStages); t--) drain(bar.vfull + t % kStages, (t / kStages) & 1);
       }
     } else if (warp == 1) {
-      if (lane == 0 && u0 < u1 && wait(&bar.qready, 0, &stop, a.derr)) {
-        constexpr uint32_t ids = idesc(DT == TCB_BF16, 0, kKeys), ido = idesc(DT == TCB_BF16, 1, HD);
-        auto s_mma = [&](int q, int st) {
-          const uint32_t qa = sa(sm + L::kQ + q * L::kTile), ka = sa(sm + L::kK + st * L::kTile);
+      // The whole warp follows the barriers and one elected thread issues, so
+      // that the descriptors stay in uniform registers.
+      constexpr uint32_t ids = idesc(DT == TCB_BF16, 0, kKeys), ido = idesc(DT == TCB_BF16, 1, HD);
+      const uint32_t base = sa(sm);
+      auto s_mma = [&](int q, int st) {
+        const uint64_t qd = desc_k(base + L::kQ + q * L::kTile), kd = desc_k(base + L::kK + st * L::kTile);
 #pragma unroll
-          for (int k = 0; k < HD / 16; k++) {
-            const uint32_t o = (k >> 2) * kHalf + (k & 3) * 32;
-            mma_ss(tmem + q * kKeys, desc_k(qa + o), desc_k(ka + o), ids, k > 0);
-          }
-          commit(bar.sfull + q);
-        };
-        bool ok = wait(bar.kfull, 0, &stop, a.derr);
-        fence_after();
-        if (ok) {
-          for (int q = 0; q < active; q++) s_mma(q, 0);
-          commit(bar.kempty);
+        for (int k = 0; k < HD / 16; k++) {
+          const uint64_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+          mma_ss(tmem + q * kKeys, qd + o, kd + o, ids, k > 0);
         }
-        for (int u = u0; u < u1 && ok; u++) {
-          const int i = u - u0, st = i % kStages, sn = (i + 1) % kStages;
-          const uint32_t ph = (i / kStages) & 1;
-          for (int q = 0; q < active && ok; q++) {
-            if (q == 0) ok = wait(bar.vready + st, ph, &stop, a.derr);
-            ok = ok && wait(bar.pready + q, i & 1, &stop, a.derr);
-            if (!ok) break;
-            fence_after();
-            const uint32_t va = sa(sm + L::kV + st * L::kTile);
+        commit(bar.sfull + q);
+      };
+      bool ok = u0 < u1 && wait_polled(&bar.qready, 0, &stop, a.derr) && wait(bar.kfull, 0, &stop, a.derr);
+      fence_after();
+      if (ok && elect()) {
+        for (int q = 0; q < active; q++) s_mma(q, 0);
+        commit(bar.kempty);
+      }
+      __syncwarp();
+      for (int u = u0; u < u1 && ok; u++) {
+        const int i = u - u0, st = i % kStages, sn = (i + 1) % kStages;
+        const uint64_t vd = desc_mn(base + L::kV + st * L::kTile);
+        ok = wait_polled(bar.vready + st, (i / kStages) & 1, &stop, a.derr);
+        if (ok && u + 1 < u1) ok = wait(bar.kfull + sn, ((i + 1) / kStages) & 1, &stop, a.derr);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; k++)
-              mma_ts(tmem + kTiles * kKeys + q * HD, tmem + q * kKeys + 8 * k, desc_mn(va + k * 2048), ido, i > 0 || k > 0);
-            commit(bar.odone + q);
-            if (q == active - 1) commit(bar.vempty + st);
+        for (int q = 0; q < kTiles; q++) {
+          if (q >= active) break;
+          // P V by halves of the positions: the first runs while the softmax
+          // forms the second
+          auto pv = [&](int half) {
+#pragma unroll
+            for (int k = 4 * half; k < 4 * half + 4; k++)
+              mma_ts(tmem + kTiles * kKeys + q * HD, tmem + q * kKeys + 8 * k, vd + (k * 2048 >> 4), ido, i > 0 || k > 0);
+          };
+          ok = ok && wait_polled(bar.phalf + q, i & 1, &stop, a.derr);
+          if (!ok) break;
+          fence_after();
+          if (elect()) pv(0);
+          __syncwarp();
+          ok = wait_polled(bar.pready + q, i & 1, &stop, a.derr);
+          if (!ok) break;
+          fence_after();
+          if (elect()) {
+            pv(1);
             // the next S goes over this P: the MMAs of one thread run in order
-            if (u + 1 < u1) {
-              if (q == 0) ok = wait(bar.kfull + sn, ((i + 1) / kStages) & 1, &stop, a.derr);
-              if (!ok) break;
-              s_mma(q, sn);
-              if (q == active - 1) commit(bar.kempty + sn);
+            if (u + 1 < u1) s_mma(q, sn);
+            commit(bar.odone + q);
+            if (q == active - 1) {
+              commit(bar.vempty + st);
+              if (u + 1 < u1) commit(bar.kempty + sn);
             }
           }
-        }
-        if (stop) {  // products in flight end before the tensor memory goes
-          commit(&bar.drained);
-          drain(&bar.drained, 0);
+          __syncwarp();
         }
       }
+      if (stop) {  // products in flight end before the tensor memory goes
+        if (elect()) commit(&bar.drained);
+        __syncwarp();
+        drain(&bar.drained, 0);
+      }
     } else {
-      // V at the edge of some row's sight
-      const int t = threadIdx.x - 64;
+      // V at the edge of some row's sight: positions that no row sees are
+      // zeroed, those that only some see are searched for non-finite elements
       bool ok = true, found = false;
       for (int u = u0; u < u1 && ok; u++) {
         const int i = u - u0, st = i % kStages;
         ok = wait(bar.vfull + st, (i / kStages) & 1, &stop, a.derr);
+        ok = __all_sync(kAll, ok);
         if (!ok) break;
         const int k0 = key_of(u);
         if (!in_full_sight(k0)) {
           uint4 *v = reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTile);
-          for (int e = t; e < L::kTile / 16; e += 64) {
-            const int pos = k0 + (e >> 3) % kKeys;  // the swizzle stays within a row's 128 bytes
-            uint4 w = v[e];
-            uint32_t *wd = &w.x;
-            bool change = false;
-            if (pos >= hi_max) {
-              w = make_uint4(0, 0, 0, 0);
-              change = true;
-            } else {
+          for (int j = (threadIdx.x - 64) >> 3; j < kKeys; j += 8) {  // a row of 128 bytes to 8 lanes; the swizzle stays within it
+            const int key = k0 + j;
+            if (key < hi_min && (key >= lo_max || key < first_min)) continue;
+            const bool none = key >= hi_max || (key < lo_min && key >= first_max);
+#pragma unroll
+            for (int h = 0; h < HD / 64; h++) {
+              uint4 *at = v + (h * kKeys + j) * 8 + (lane & 7);
+              if (none) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              const uint4 w = *at;
+              uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+              bool change = false;
 #pragma unroll
               for (int d = 0; d < 4; d++)
                 if (nonfinite2<DT>(wd[d])) {
                   if (nonfinite2<DT>(wd[d] & 0xFFFFu)) wd[d] &= 0xFFFF0000u;
                   if (nonfinite2<DT>(wd[d] & 0xFFFF0000u)) wd[d] &= 0xFFFFu;
-                  change = found = true;
+                  change = true;
                 }
+              if (change) {
+                *at = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+                found = true;
+              }
             }
-            if (change) v[e] = w;
           }
-          if (found) dirty = 1;
           mv::fence_proxy_async();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar.vready + st);
       }
+      if (found) dirty = 1;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.checked);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // Q into the swizzled tile (rows that do not exist are zero)
     if (qt < active) {
       const uint16_t *q = static_cast<const uint16_t *>(a.q) + r * a.ldq + (long)head * HD;
@@ -439,7 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     if (qt < active) {
       const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
       const uint32_t ts_addr = tmem + lanes + qt * kKeys, to_addr = tmem + lanes + kTiles * kKeys + qt * HD;
-      float m = -INFINITY, l = 0.f;  // m in scaled units
+      float m = -INFINITY;           // in scaled units
+      uint64_t l0 = 0ull, l1 = 0ull;  // the sum, in four parts
       bool ok = true;
       for (int u = u0; u < u1; u++) {
         const int i = u - u0, k0 = key_of(u);
@@ -452,16 +535,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         tmem_wait_ld();
         if (!in_full_sight(k0)) {
 #pragma unroll
-          for (int j = 0; j < kKeys; j++) {
-            const int key = k0 + j;
-            if (key >= hi || (key < lo && key >= first)) s[j] = 0xFF800000u;
+          for (int c = 0; c < 4; c++) {
+            const int at = k0 + 32 * c;
+            const uint32_t seen = below(hi - at) & (~below(lo - at) | below(first - at));
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              if (!(seen >> j & 1)) s[32 * c + j] = 0xFF800000u;
           }
         }
-        float top = __uint_as_float(s[0]);
+        auto sf = [&](int j) { return __uint_as_float(s[j]); };
+        float tops[4];
 #pragma unroll
-        for (int j = 1; j < kKeys; j++) top = fmaxf(top, __uint_as_float(s[j]));
-        top *= scale;
-        const bool up = top > m + kSlack;
+        for (int c = 0; c < 4; c++) {
+          tops[c] = max3_nan(sf(c), sf(c + 4), sf(c + 8));
+#pragma unroll
+          for (int j = c + 12; j < kKeys; j += 8) tops[c] = max3_nan(tops[c], sf(j), j + 4 < kKeys ? sf(j + 4) : sf(j));
+        }
+        float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * scale;
+        if (!(top < INFINITY)) top = NAN;  // infinite and NaN scores make the row NaN
+        const bool up = top > m + kSlack || top != top;
         if (i == 0) {
           if (up) m = top;
         } else if (__any_sync(kAll, up)) {
@@ -469,11 +561,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
           ok = wait(bar.odone + qt, (i - 1) & 1, &stop, a.derr);
           if (!__all_sync(kAll, ok)) break;
           fence_after();
-          const float keep = up ? (m == -INFINITY ? 0.f : exp2f(m - top)) : 1.f;
-          if (up) {
-            m = top;
-            l *= keep;
-          }
+          // every row of the warp takes its new maximum, so that the next
+          // time is far off
+          const float next = top > m || up ? top : m;
+          const float keep = next == m ? 1.f : m == -INFINITY ? 0.f : exp2f(m - next);
+          m = next;
+          l0 = fma2(l0, pair(keep, keep), 0ull);
+          l1 = fma2(l1, pair(keep, keep), 0ull);
 #pragma unroll 1
           for (int c = 0; c < HD / 32; c++) {
             uint32_t o[32];
@@ -486,28 +580,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
           tmem_wait_st();
         }
         const float sub = m == -INFINITY ? 0.f : m;
+        const uint64_t mul = pair(scale, scale), off = pair(-sub, -sub);
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           uint32_t pk[32];
 #pragma unroll
           for (int j = 0; j < 32; j++) {
-            const float p0 = exp2_fast(fmaf(__uint_as_float(s[64 * c + 2 * j]), scale, -sub));
-            const float p1 = exp2_fast(fmaf(__uint_as_float(s[64 * c + 2 * j + 1]), scale, -sub));
-            l += p0 + p1;
-            pk[j] = pack2<DT>(p0, p1);
+            const uint64_t x = fma2(pair(sf(64 * c + 2 * j), sf(64 * c + 2 * j + 1)), mul, off);
+            float2 w = split2(x);
+            w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+            if (j & 1) l1 = add2(l1, pair(w.x, w.y));
+            else l0 = add2(l0, pair(w.x, w.y));
+            pk[j] = pack2<DT>(w.x, w.y);
           }
           tmem_st(ts_addr + 32 * c, pk);
+          tmem_wait_st();
+          fence_before();
+          mbar_arrive((c ? bar.pready : bar.phalf) + qt);
         }
-        tmem_wait_st();
-        fence_before();
-        mbar_arrive(bar.pready + qt);
       }
       const int iters = u1 - u0;
       if (iters > 0 && ok) ok = wait(bar.odone + qt, (iters - 1) & 1, &stop, a.derr);
       if (ok) ok = wait(&bar.checked, 0, &stop, a.derr);
       ok = __all_sync(kAll, ok);
       fence_after();
-      const bool empty = iters == 0 || l == 0.f;
+      const float2 la = split2(l0), lb = split2(l1);
+      const float l = (la.x + la.y) + (lb.x + lb.y);
+      const bool empty = iters == 0 || m == -INFINITY;
       const float inv = p.po ? 1.f : __fdiv_rn(1.f, empty ? 1.f : l);
       const long prow = ((long)part * a.T + r) * a.H + head;
       if (p.po && live) p.pml[prow] = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
