@@ -21,7 +21,7 @@ import math
 
 import torch
 
-from . import BF16, F16, F32, TcbError, _stream, lib
+from . import BF16, F16, F32, TcbError, lib
 
 _TYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _I32, _I64 = torch.int32, torch.int64
@@ -44,6 +44,13 @@ class _LogitsArgs(ctypes.Structure):
                 ("bias_ids", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("n_bias", ctypes.c_int), ("ldb", ctypes.c_long),
                 ("mask", ctypes.c_void_p), ("n_masks", ctypes.c_int), ("ldm", ctypes.c_long),
                 ("mask_row", ctypes.c_void_p)]
+
+
+def _stream(ctx, stream) -> int:
+    """The handle of `stream`, or of the current stream of the context's device."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(ctx.device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 _bound = None
@@ -70,16 +77,19 @@ def _need(ok: bool, what: str):
 
 def _vec(t, n: int, dtype, name: str) -> int:
     """Address of a contiguous device vector of at least n elements."""
-    if t.dtype != dtype or not t.is_cuda or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+    if t.dtype is not dtype or not t.is_cuda or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous {dtype} CUDA vector of at least {n} elements is wanted")
     return t.data_ptr()
 
 
 def _rows(t, dtype, name: str):
     """(address, width, row stride) of a 2-D device tensor with dense rows."""
-    if t.dtype != dtype or not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dtype is not dtype or not t.is_cuda or t.dim() != 2:
         raise ValueError(f"{name}: a 2-D {dtype} CUDA tensor with dense rows is wanted")
-    return t.data_ptr(), t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    (n, width), (ld, unit) = t.shape, t.stride()
+    if width > 1 and unit != 1:
+        raise ValueError(f"{name}: a 2-D {dtype} CUDA tensor with dense rows is wanted")
+    return t.data_ptr(), width, ld if n > 1 else width
 
 
 def plan(ctx, page, cached, fresh, tables, free, n_free, row_start, kv_len, slots, positions, balance, taken=None,
@@ -97,7 +107,7 @@ def plan(ctx, page, cached, fresh, tables, free, n_free, row_start, kv_len, slot
                               rows, _vec(row_start, B + 1, _I32, "row_start"), _vec(kv_len, B, _I32, "kv_len"),
                               _vec(slots, 0, _I64, "slots"), _vec(positions, rows, _I32, "positions"),
                               _vec(balance, 1, _I32, "balance"),
-                              0 if taken is None else _vec(taken, 1, _I32, "taken"), _stream(stream))
+                              0 if taken is None else _vec(taken, 1, _I32, "taken"), _stream(ctx, stream))
     ctx._check(rc, "tcb_page_plan")
 
 
@@ -130,7 +140,7 @@ class Pages:
         if k.dtype not in _TYPE:
             raise TcbError(2, "tcb_kv_append")
         rc = _lib().tcb_kv_append(self.ctx.handle, self._ref, T, k.data_ptr(), v.data_ptr(), _TYPE[k.dtype],
-                                  k.stride(0) if T > 1 else n, _vec(slots, T, _I64, "slots"), _stream(stream))
+                                  k.stride(0) if T > 1 else n, _vec(slots, T, _I64, "slots"), _stream(self.ctx, stream))
         self.ctx._check(rc, "tcb_kv_append")
 
     def _q(self, q, out):
@@ -156,7 +166,7 @@ class Pages:
         rc = _lib().tcb_page_attn(self.ctx.handle, self._ref, B, T, H, qp, ldq, op, ldo,
                                   _vec(row_start, B + 1, _I32, "row_start"), _vec(kv_len, B, _I32, "kv_len"), tp, width,
                                   ldt, max_rows, max_len, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-                                  -1 if window is None else window, sinks, _stream(stream))
+                                  -1 if window is None else window, sinks, _stream(self.ctx, stream))
         self.ctx._check(rc, "tcb_page_attn")
         return out
 
@@ -170,7 +180,7 @@ class Pages:
         rc = _lib().tcb_prefix_attn(self.ctx.handle, self._ref, T, H, qp, ldq, op, ldo,
                                     _vec(prefix, -(-prefix_len // self.page), _I32, "prefix"), prefix_len,
                                     _vec(kv_len, T, _I32, "kv_len"), tp, width, ldt, max_len,
-                                    1.0 / math.sqrt(self.head_dim) if scale is None else scale, _stream(stream))
+                                    1.0 / math.sqrt(self.head_dim) if scale is None else scale, _stream(self.ctx, stream))
         self.ctx._check(rc, "tcb_prefix_attn")
         return out
 
@@ -213,6 +223,6 @@ def penalize(ctx, logits, out, token=None, history=None, prompt_len=None, total_
                     _vec(presence, B, f32, "presence") if presence is not None else 0,
                     ip, vp, nb, ldb, mp, nm, ldm,
                     _vec(mask_row, B, _I32, "mask_row") if mask_row is not None else 0)
-    rc = _lib().tcb_logits_penalize(ctx.handle, ctypes.byref(a), _stream(stream))
+    rc = _lib().tcb_logits_penalize(ctx.handle, ctypes.byref(a), _stream(ctx, stream))
     ctx._check(rc, "tcb_logits_penalize")
     return out
