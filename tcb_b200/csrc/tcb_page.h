@@ -52,6 +52,7 @@ struct DecodePlan {
   size_t o_bytes, bytes;  // scratch of the join across clusters
   size_t counters;        // bytes of zeroed counters
 };
+constexpr int kMaxPrefixParts = 64;
 struct PrefixPartials {
   int parts;
   const float *o;

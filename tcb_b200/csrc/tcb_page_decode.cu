@@ -40,6 +40,7 @@
 #include <algorithm>
 
 #include "tcb_common.cuh"
+#include "tcb_mv_ptx.cuh"
 #include "tcb_page.h"
 
 namespace tcb {
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   __shared__ float so[kWarps][Q][HD];
   __shared__ float sm[kWarps][Q], sl[kWarps][Q];
   __shared__ float cm[Q], cl[Q];  // the CTA's
+  __shared__ float xm[Q], xl[Q], xg[kMaxPrefixParts][Q];  // the prefix's partials: maximum, sum, weights
   const int G = a.H / a.kv.n_kv_heads, tiles = (G + Q - 1) / Q;
   const int kh = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * Q;  // first query head within the group
   const int b = blockIdx.z, n_cta = gridDim.x;
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
             make_float2(o[d][x][e], o[d][x][2 + e]);
     }
   __syncthreads();
-  const int per_row = HD / 2;  // pairs of elements
+  constexpr int per_row = HD / 2;  // pairs of elements
   for (int i = threadIdx.x; i < Q * per_row; i += kThreads) {
     const int q = i / per_row, d = 2 * (i - q * per_row);
     float top = sm[0][q];
@@ -346,51 +348,95 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   }
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
+  if (x.parts) {
+    // the prefix's partials are complete; per query their joint maximum, sum and
+    // weights, 128 / Q lanes a query
+    mv::pdl_wait();
+    constexpr int lanes = kThreads / Q;
+    const int q = threadIdx.x / lanes, at = threadIdx.x % lanes;
+    const float2 *ml = x.ml + (long)r * a.H + kh * G + min(h0 + q, G - 1);
+    const long all_rows = (long)a.T * a.H;
+    float top = -INFINITY, sum = 0.f;
+    for (int w = at; w < x.parts; w += lanes) top = fmaxf(top, __ldcg(ml + w * all_rows).x);
+#pragma unroll
+    for (int w = 1; w < lanes; w <<= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, w));
+    for (int w = at; w < x.parts; w += lanes) {
+      const float2 v = __ldcg(ml + w * all_rows);
+      const float g = join_weight(v.x, top);
+      xg[w][q] = g;
+      sum += g * v.y;
+    }
+#pragma unroll
+    for (int w = 1; w < lanes; w <<= 1) sum += __shfl_xor_sync(kAll, sum, w);
+    if (at == 0) xm[q] = top, xl[q] = sum;
+  }
   if (n_rank > 1) cluster.sync();
   else __syncthreads();
   // this rank's slice of the outputs, over the cluster's partials in rank order
-  const int live_q = min(Q, G - h0), all = live_q * per_row;
+  const int live_q = min(Q, G - h0);
   uint16_t *out = static_cast<uint16_t *>(a.out) + r * a.ldo + (long)(kh * G + h0) * HD;
-  auto store = [&](int q, int d, float2 acc, float top, float sum) {
-    if (x.parts) {  // the prefix, in the order of its parts
-      const long row = (long)r * a.H + kh * G + h0 + q, all_rows = (long)a.T * a.H;
-      float joint = top;
-      for (int w = 0; w < x.parts; w++) joint = fmaxf(joint, __ldcg(x.ml + w * all_rows + row).x);
-      const float f = join_weight(top, joint);
-      acc.x *= f, acc.y *= f, sum *= f;
-      for (int w = 0; w < x.parts; w++) {
-        const float2 ml = __ldcg(x.ml + w * all_rows + row);
-        const float2 v = __ldcg(reinterpret_cast<const float2 *>(x.o + (w * all_rows + row) * HD + d));
-        const float g = join_weight(ml.x, joint);
-        acc.x += g * v.x, acc.y += g * v.y, sum += g * ml.y;
+  // a thread's element pairs: its i-th is number (i * n_rank + c) * kThreads + threadIdx.x
+  constexpr int kItems = Q * per_row / kThreads;
+  auto query_of = [&](int i) { return ((i * n_rank + c) * kThreads + (int)threadIdx.x) / per_row; };
+  const int d = 2 * ((int)threadIdx.x % per_row);
+  auto store = [&](float2 (&acc)[kItems], float (&top)[kItems], float (&sum)[kItems]) {
+    if (x.parts) {  // the prefix's part, in the order of its partials
+      const long all_rows = (long)a.T * a.H, row0 = (long)r * a.H + kh * G + h0;
+      float2 pre[kItems];
+#pragma unroll
+      for (int i = 0; i < kItems; i++) pre[i] = make_float2(0.f, 0.f);
+#pragma unroll 4
+      for (int w = 0; w < x.parts; w++)
+#pragma unroll
+        for (int i = 0; i < kItems; i++) {
+          const int q = query_of(i);
+          if (q >= live_q) continue;
+          const float2 v = __ldcg(reinterpret_cast<const float2 *>(x.o + (w * all_rows + row0 + q) * HD + d));
+          pre[i].x += xg[w][q] * v.x, pre[i].y += xg[w][q] * v.y;
+        }
+#pragma unroll
+      for (int i = 0; i < kItems; i++) {
+        const int q = query_of(i);
+        if (q >= live_q) continue;
+        const float joint = fmaxf(top[i], xm[q]), f = join_weight(top[i], joint), g = join_weight(xm[q], joint);
+        acc[i].x = f * acc[i].x + g * pre[i].x, acc[i].y = f * acc[i].y + g * pre[i].y;
+        sum[i] = f * sum[i] + g * xl[q];
       }
     }
-    float v0 = sum == 0.f ? 0.f : __fdiv_rn(acc.x, sum), v1 = sum == 0.f ? 0.f : __fdiv_rn(acc.y, sum);
-    *reinterpret_cast<uint32_t *>(out + (long)q * HD + d) = pack2<DT>(v0, v1);
+#pragma unroll
+    for (int i = 0; i < kItems; i++) {
+      const int q = query_of(i);
+      if (q >= live_q) continue;
+      float v0 = sum[i] == 0.f ? 0.f : __fdiv_rn(acc[i].x, sum[i]), v1 = sum[i] == 0.f ? 0.f : __fdiv_rn(acc[i].y, sum[i]);
+      *reinterpret_cast<uint32_t *>(out + (long)q * HD + d) = pack2<DT>(v0, v1);
+    }
   };
   const long unit = (long)blockIdx.z * gridDim.y + blockIdx.y;
   auto part_o = [&](int w, int q, int d) {
     return reinterpret_cast<float2 *>(j.o + ((unit * j.parts + w) * Q + q) * HD + d);
   };
   auto part_ml = [&](int w, int q) { return j.ml + ((unit * j.parts + w) * n_rank + c) * Q + q; };
-  for (int i = c * kThreads + threadIdx.x; i < all; i += n_rank * kThreads) {
-    const int q = i / per_row, d = 2 * (i - q * per_row);
-    float top = -INFINITY, sum = 0.f;
-    float2 acc = make_float2(0.f, 0.f);
-    for (int w = 0; w < n_rank; w++) top = fmaxf(top, *cluster.map_shared_rank(&cm[q], w));
+  float2 acc[kItems];
+  float top[kItems], sum[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; i++) {
+    const int q = query_of(i);
+    acc[i] = make_float2(0.f, 0.f);
+    top[i] = -INFINITY, sum[i] = 0.f;
+    if (q >= live_q) continue;
+    for (int w = 0; w < n_rank; w++) top[i] = fmaxf(top[i], *cluster.map_shared_rank(&cm[q], w));
     for (int w = 0; w < n_rank; w++) {
-      const float f = join_weight(*cluster.map_shared_rank(&cm[q], w), top);
+      const float f = join_weight(*cluster.map_shared_rank(&cm[q], w), top[i]);
       const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&so[0][q][d], w));
-      acc.x += f * v.x, acc.y += f * v.y;
-      sum += f * *cluster.map_shared_rank(&cl[q], w);
+      acc[i].x += f * v.x, acc[i].y += f * v.y;
+      sum[i] += f * *cluster.map_shared_rank(&cl[q], w);
     }
-    if (j.parts == 1) {
-      store(q, d, acc, top, sum);
-    } else {
-      __stcg(part_o(part, q, d), acc);
-      __stcg(part_ml(part, q), make_float2(top, sum));  // the same value from every thread of the query
+    if (j.parts > 1) {
+      __stcg(part_o(part, q, d), acc[i]);
+      __stcg(part_ml(part, q), make_float2(top[i], sum[i]));  // the same value from every thread of the query
     }
   }
+  if (j.parts == 1) store(acc, top, sum);
   if (n_rank > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
   if (j.parts == 1) return;
   // the last of the clusters' ranks c joins their slices, in cluster order
@@ -405,19 +451,22 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   __syncthreads();
   if (!last) return;
   __threadfence();
-  for (int i = c * kThreads + threadIdx.x; i < all; i += n_rank * kThreads) {
-    const int q = i / per_row, d = 2 * (i - q * per_row);
-    float top = -INFINITY, sum = 0.f;
-    float2 acc = make_float2(0.f, 0.f);
-    for (int w = 0; w < j.parts; w++) top = fmaxf(top, __ldcg(part_ml(w, q)).x);
+#pragma unroll
+  for (int i = 0; i < kItems; i++) {
+    const int q = query_of(i);
+    acc[i] = make_float2(0.f, 0.f);
+    top[i] = -INFINITY, sum[i] = 0.f;
+    if (q >= live_q) continue;
+    for (int w = 0; w < j.parts; w++) top[i] = fmaxf(top[i], __ldcg(part_ml(w, q)).x);
+#pragma unroll 4
     for (int w = 0; w < j.parts; w++) {
       const float2 ml = __ldcg(part_ml(w, q)), v = __ldcg(part_o(w, q, d));
-      const float f = join_weight(ml.x, top);
-      acc.x += f * v.x, acc.y += f * v.y;
-      sum += f * ml.y;
+      const float f = join_weight(ml.x, top[i]);
+      acc[i].x += f * v.x, acc[i].y += f * v.y;
+      sum[i] += f * ml.y;
     }
-    store(q, d, acc, top, sum);
   }
+  store(acc, top, sum);
 }
 
 template <int DT, int HD, int NT>
@@ -426,12 +475,15 @@ cudaError_t launch(const PageAttnArgs &a, const DecodePlan &pl, const Join &j, c
   cfg.gridDim = dim3(pl.split, pl.units / a.B, a.B);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = j.ranks;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  // behind the prefix's kernel: the suffixes are read while it runs
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = x.parts ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k_page_decode<DT, HD, NT>, a, j, x);
 }
 

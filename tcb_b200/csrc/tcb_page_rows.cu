@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     n = min(n, a.max_rows);
   }
   const long x0 = (long)tile * kTiles * kRows, rows = (long)n * p.G;
+  if (p.joined) mv::pdl_launch_dependents();  // the kernel of the suffixes, which waits before it reads the partials
   if (x0 >= rows) return;
   const int n_real = p.joined ? n : min(max(a.row_start[b + 1], r0), a.T) - r0;  // positions count from the true number of rows
   const int active = rows - x0 > kRows ? 2 : 1;  // query tiles with rows
@@ -731,6 +732,7 @@ RowsPlan page_rows_plan(const PageAttnArgs &a) {
   const long keys = (seen + pr::kKeys - 1) / pr::kKeys, units = (long)pl.tiles * a.kv.n_kv_heads * (joined ? 1 : a.B);
   // CTAs along the positions where the others leave SMs idle, two tiles each at the least
   pl.split = (int)std::max<long>(1, std::min<long>(148 / units, keys / 2));
+  if (joined) pl.split = std::min(pl.split, kMaxPrefixParts);
   pl.partial = joined || pl.split > 1;
   if (pl.partial) {
     const size_t n = (size_t)pl.split * a.T * a.H;
