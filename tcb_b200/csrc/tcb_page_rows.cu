@@ -127,7 +127,11 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t *r) {
       TCB_W8(r, 8), TCB_W8(r, 16), TCB_W8(r, 24), "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// waits for the loads; r (32 words) is used after it
+#define TCB_X8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : TCB_X8(r, 0), TCB_X8(r, 8), TCB_X8(r, 16), TCB_X8(r, 24)::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *tm, int x, int pos, int head, int page,
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     if (bad) len = 0;
     n = min(n, a.max_rows);
   }
-  const long x0 = (long)tile * kTiles * kRows, rows = (long)n * p.G;
+  const int x0 = tile * kTiles * kRows, rows = n * p.G;  // (row, head) pairs: fewer than the bytes of q
   if (p.joined) mv::pdl_launch_dependents();  // the kernel of the suffixes, which waits before it reads the partials
   if (x0 >= rows) return;
   const int n_real = p.joined ? n : min(max(a.row_start[b + 1], r0), a.T) - r0;  // positions count from the true number of rows
@@ -305,10 +309,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
 
   // softmax threads: the row, what it sees, and its Q
   const int qt = (warp >> 2) - 1, tid = threadIdx.x & 127;  // warps 4-7: 0, 8-11: 1
-  const long x = x0 + qt * kRows + tid;
+  const int x = x0 + qt * kRows + tid;
   const bool live = qt >= 0 && x < rows;
-  const int xi = live ? (int)(x / p.G) : 0;
-  const int head = kh * p.G + (live ? (int)(x - (long)xi * p.G) : 0);
+  const int xi = live ? (int)((unsigned)x / (unsigned)p.G) : 0;
+  const int head = kh * p.G + (live ? x - xi * p.G : 0);
   const long r = r0 + xi;
   int hi = 0, lo = 0, first = 0;
   if (live) {
@@ -504,17 +508,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // Q into the swizzled tile (rows that do not exist are zero)
+    // Q into the swizzled tile (rows that do not exist are zero): the warp takes
+    // its 32 rows one after the other, HD / 8 lanes a row
     if (qt < active) {
-      const uint16_t *q = static_cast<const uint16_t *>(a.q) + r * a.ldq + (long)head * HD;
-      uint8_t *dst = sm + L::kQ + qt * L::kTile + tid * 128;
+      const long at = live && a.scale_log2 != 0.f ? r * a.ldq + (long)head * HD : -1;
       const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+      constexpr int kLanes = HD / 8;
+      const int c = lane % kLanes;
+      uint4 v[kLanes];
 #pragma unroll
-      for (int c = 0; c < HD / 8; c++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live && a.scale_log2 != 0.f) v = *reinterpret_cast<const uint4 *>(q + 8 * c);
-        v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
-        *reinterpret_cast<uint4 *>(dst + (c >> 3) * kHalf + (((c & 7) ^ (tid & 7)) << 4)) = v;
+      for (int i = 0; i < kLanes; i++) {
+        const long off = __shfl_sync(kAll, at, i * (32 / kLanes) + lane / kLanes);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (off >= 0) v[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + off + 8 * c);
+      }
+#pragma unroll
+      for (int i = 0; i < kLanes; i++) {
+        const int row = (warp & 3) * 32 + i * (32 / kLanes) + lane / kLanes;
+        v[i].x ^= sign, v[i].y ^= sign, v[i].z ^= sign, v[i].w ^= sign;
+        *reinterpret_cast<uint4 *>(sm + L::kQ + qt * L::kTile + row * 128 + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)) = v[i];
       }
       mv::fence_proxy_async();
     }
@@ -533,7 +545,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         uint32_t s[kKeys];
 #pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld(ts_addr + 32 * c, s + 32 * c);
-        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_wait_ld(s + 32 * c);
         if (!in_full_sight(k0)) {
 #pragma unroll
           for (int c = 0; c < 4; c++) {
@@ -573,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
           for (int c = 0; c < HD / 32; c++) {
             uint32_t o[32];
             tmem_ld(to_addr + 32 * c, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
             tmem_st(to_addr + 32 * c, o);
@@ -616,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         uint32_t o[32];
         if (iters > 0) {
           tmem_ld(to_addr + 32 * c, o);
-          tmem_wait_ld();
+          tmem_wait_ld(o);
         }
 #pragma unroll
         for (int j = 0; j < 32; j++) o[j] = empty ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
@@ -643,20 +656,37 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
             }
           }
         }
-        if (!live) continue;
+        // through this warp's part of the Q tile (its products are done), so that
+        // whole sectors are written
+        uint8_t *stage = sm + L::kQ + qt * L::kTile + (warp & 3) * 4096;
+        __syncwarp();
         if (p.po) {
-          float4 *dst = reinterpret_cast<float4 *>(p.po + prow * HD + 32 * c);
 #pragma unroll
           for (int j = 0; j < 8; j++)
-            dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+            *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int row = 4 * i + (lane >> 3), j = lane & 7;
+            const long to = __shfl_sync(kAll, live ? prow : -1, row);
+            if (to >= 0) *reinterpret_cast<uint4 *>(p.po + to * HD + 32 * c + 4 * j) = *reinterpret_cast<const uint4 *>(stage + row * 128 + ((j ^ (row & 7)) << 4));
+          }
         } else {
-          uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + r * a.ldo + (long)head * HD + 32 * c);
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) w[e] = pack2<DT>(__uint_as_float(o[8 * j + 2 * e]), __uint_as_float(o[8 * j + 2 * e + 1]));
-            dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+          const long out_row = live ? r * a.ldo + (long)head * HD : -1;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int row = 8 * i + (lane >> 2), j = lane & 3;
+            const long to = __shfl_sync(kAll, out_row, row);
+            if (to >= 0)
+              *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to + 32 * c + 8 * j) = *reinterpret_cast<const uint4 *>(stage + row * 64 + ((j ^ (row >> 1 & 3)) << 4));
           }
         }
       }
