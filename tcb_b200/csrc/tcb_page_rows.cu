@@ -154,19 +154,6 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase, volatile int
   atomicExch(err, TCB_ERR_TIMEOUT);
   return false;
 }
-// A barrier that other warps arrive on: a suspended try_wait wakes late from
-// those (about 700 cycles), so it is polled (with or without the sleep is the
-// same time).
-__device__ __forceinline__ bool wait_polled(uint64_t *bar, uint32_t phase, volatile int *stop, int *err) {
-  for (uint32_t i = 0; i < 1u << 26; i++) {
-    if (mv::mbar_test_wait(bar, phase)) return true;
-    if (*stop) return false;
-    __nanosleep(32);
-  }
-  *stop = 1;
-  atomicExch(err, TCB_ERR_TIMEOUT);
-  return false;
-}
 // one thread of a converged warp
 __device__ __forceinline__ bool elect() {
   uint32_t p;
@@ -410,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         }
         commit(bar.sfull + q);
       };
-      bool ok = u0 < u1 && wait_polled(&bar.qready, 0, &stop, a.derr) && wait(bar.kfull, 0, &stop, a.derr);
+      bool ok = u0 < u1 && wait(&bar.qready, 0, &stop, a.derr) && wait(bar.kfull, 0, &stop, a.derr);
       fence_after();
       if (ok && elect()) {
         for (int q = 0; q < active; q++) s_mma(q, 0);
@@ -420,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       for (int u = u0; u < u1 && ok; u++) {
         const int i = u - u0, st = i % kStages, sn = (i + 1) % kStages;
         const uint64_t vd = desc_mn(base + L::kV + st * L::kTile);
-        ok = wait_polled(bar.vready + st, (i / kStages) & 1, &stop, a.derr);
+        ok = wait(bar.vready + st, (i / kStages) & 1, &stop, a.derr);
         if (ok && u + 1 < u1) ok = wait(bar.kfull + sn, ((i + 1) / kStages) & 1, &stop, a.derr);
 #pragma unroll
         for (int q = 0; q < kTiles; q++) {
@@ -432,12 +419,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
             for (int k = 4 * half; k < 4 * half + 4; k++)
               mma_ts(tmem + kTiles * kKeys + q * HD, tmem + q * kKeys + 8 * k, vd + (k * 2048 >> 4), ido, i > 0 || k > 0);
           };
-          ok = ok && wait_polled(bar.phalf + q, i & 1, &stop, a.derr);
+          ok = ok && wait(bar.phalf + q, i & 1, &stop, a.derr);
           if (!ok) break;
           fence_after();
           if (elect()) pv(0);
           __syncwarp();
-          ok = wait_polled(bar.pready + q, i & 1, &stop, a.derr);
+          ok = wait(bar.pready + q, i & 1, &stop, a.derr);
           if (!ok) break;
           fence_after();
           if (elect()) {
@@ -469,30 +456,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         if (!ok) break;
         const int k0 = key_of(u);
         if (!in_full_sight(k0)) {
-          uint4 *v = reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTile);
-          for (int j = (threadIdx.x - 64) >> 3; j < kKeys; j += 8) {  // a row of 128 bytes to 8 lanes; the swizzle stays within it
-            const int key = k0 + j;
+          // 8 lanes a row of 128 bytes (the swizzle stays within it), 8 rows at a time
+          uint4 *v = reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTile) + (threadIdx.x - 64);
+          constexpr uint32_t e = DT == TCB_F16 ? 0x7C007C00u : 0x7F807F80u, one = DT == TCB_F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll 4
+          for (int j0 = 0; j0 < kKeys; j0 += 8) {
+            const int key = k0 + j0 + ((threadIdx.x - 64) >> 3);
             if (key < hi_min && (key >= lo_max || key < first_min)) continue;
             const bool none = key >= hi_max || (key < lo_min && key >= first_max);
 #pragma unroll
             for (int h = 0; h < HD / 64; h++) {
-              uint4 *at = v + (h * kKeys + j) * 8 + (lane & 7);
+              uint4 *at = v + (h * kKeys + j0) * 8;
+              uint4 w = *at;
+              // an exponent of ones carries into the sign's place
+              const uint32_t bad = ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one);
               if (none) {
                 *at = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              const uint4 w = *at;
-              uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-              bool change = false;
+              } else if (bad & 0x80008000u) {
+                uint32_t *wd = &w.x;
 #pragma unroll
-              for (int d = 0; d < 4; d++)
-                if (nonfinite2<DT>(wd[d])) {
-                  if (nonfinite2<DT>(wd[d] & 0xFFFFu)) wd[d] &= 0xFFFF0000u;
-                  if (nonfinite2<DT>(wd[d] & 0xFFFF0000u)) wd[d] &= 0xFFFFu;
-                  change = true;
+                for (int d = 0; d < 4; d++) {
+                  const uint32_t b = ((wd[d] & e) + one) & 0x80008000u;
+                  wd[d] &= ~((b >> 15) * 0xFFFFu);
                 }
-              if (change) {
-                *at = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+                *at = w;
                 found = true;
               }
             }
