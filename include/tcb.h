@@ -366,14 +366,14 @@ int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached,
                   int rows, int *row_start, int *kv_len, int64_t *slots,
                   int *positions, int *balance, int *taken, void *stream);
 
-/* Append T rows of K and V (row r, head h at k + r * ldx + h * head_dim, and
- * v alike; F32, F16 or BF16) to the cache: row r goes to slot
+/* Append T rows of K and V (row r, head h at k + r * ldk + h * head_dim and
+ * v + r * ldv + h * head_dim; F32, F16 or BF16) to the cache: row r goes to slot
  * slots[r] = page number * page + position in the page, rounded once to the
  * cache's type.  Rows with a negative slot are dropped.  Of two rows with one
  * slot either may stay. */
 int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k,
-                  const void *v, int xdtype, long ldx, const int64_t *slots,
-                  void *stream);
+                  long ldk, const void *v, long ldv, int xdtype,
+                  const int64_t *slots, void *stream);
 
 /* Attention of B requests over their pages, causal, with a sliding window
  * and first positions that stay visible:

@@ -204,7 +204,8 @@ __device__ __forceinline__ uint4 load_cache8(const void *x, long i, int dtype) {
 constexpr int kAppendThreads = 256, kAppendRows = 4;
 template <int XT, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const tcb_kv_pages kv, int page_shift, int T, const void *k,
-                                                              const void *v, long ldx, const int64_t *slots, int *derr) {
+                                                              long ldk, const void *v, long ldv, const int64_t *slots,
+                                                              int *derr) {
   const int per_head = kv.head_dim / 8, places = kv.n_kv_heads * per_head;
   const int across = min(places, kAppendThreads);  // threads along a row; the CTA's other threads take other rows
   const int c = blockIdx.y * across + threadIdx.x % across, sub = threadIdx.x / across, rows = kAppendThreads / across;
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const tcb_kv_pages
 #pragma unroll
     for (int i = 0; i < kAppendRows; i++)
       if (r0 + i * step < T) {
-        kx[i] = load_cache8<XT, VEC>(k, (r0 + i * step) * ldx + x0, kv.dtype);
-        vx[i] = load_cache8<XT, VEC>(v, (r0 + i * step) * ldx + x0, kv.dtype);
+        kx[i] = load_cache8<XT, VEC>(k, (r0 + i * step) * ldk + x0, kv.dtype);
+        vx[i] = load_cache8<XT, VEC>(v, (r0 + i * step) * ldv + x0, kv.dtype);
       }
 #pragma unroll
     for (int i = 0; i < kAppendRows; i++) {
@@ -308,27 +309,27 @@ int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached, const int *f
   return e == cudaSuccess ? TCB_OK : tcb::ctx_fail(ctx, e);
 }
 
-int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k, const void *v, int xdtype, long ldx,
-                  const int64_t *slots, void *stream) {
+int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k, long ldk, const void *v, long ldv,
+                  int xdtype, const int64_t *slots, void *stream) {
   if (!ctx) return TCB_ERR_NULL;
   int rc = check_pages(kv);
   if (rc != TCB_OK) return rc;
   if (xdtype != TCB_F32 && xdtype != TCB_F16 && xdtype != TCB_BF16) return TCB_ERR_DTYPE;
   if (T < 0) return TCB_ERR_SHAPE;
   if (T == 0) return TCB_OK;
-  if (ldx < (long)kv->n_kv_heads * kv->head_dim) return TCB_ERR_SHAPE;
+  if (std::min(ldk, ldv) < (long)kv->n_kv_heads * kv->head_dim) return TCB_ERR_SHAPE;
   if (!k || !v || !slots) return TCB_ERR_NULL;
   const size_t xe = xdtype == TCB_F32 ? 4 : 2;
   if (!aligned(k, xe) || !aligned(v, xe) || !aligned(slots, 8)) return TCB_ERR_ALIGN;
   if ((rc = tcb::ctx_bind(ctx)) != TCB_OK) return rc;
-  const bool vec = aligned(k, 16) && aligned(v, 16) && ldx * (long)xe % 16 == 0;
+  const bool vec = aligned(k, 16) && aligned(v, 16) && (ldk | ldv) * (long)xe % 16 == 0;
   const int places = kv->n_kv_heads * (kv->head_dim / 8), across = std::min(places, kAppendThreads);
   const long rows = kAppendThreads / across, waves = (T + rows - 1) / rows;
   const int most = 8 * ctx->sms;
   const dim3 grid((unsigned)std::min<long>(waves, most), (unsigned)((places + across - 1) / across));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sh = log2i(kv->page);
-  auto go = [&](auto kernel) { kernel<<<grid, kAppendThreads, 0, s>>>(*kv, sh, T, k, v, ldx, slots, ctx->derr); };
+  auto go = [&](auto kernel) { kernel<<<grid, kAppendThreads, 0, s>>>(*kv, sh, T, k, ldk, v, ldv, slots, ctx->derr); };
   if (xdtype == TCB_F32) vec ? go(k_kv_append<TCB_F32, true>) : go(k_kv_append<TCB_F32, false>);
   else if (xdtype == TCB_F16) vec ? go(k_kv_append<TCB_F16, true>) : go(k_kv_append<TCB_F16, false>);
   else vec ? go(k_kv_append<TCB_BF16, true>) : go(k_kv_append<TCB_BF16, false>);

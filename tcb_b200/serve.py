@@ -62,7 +62,7 @@ def _lib():
         L = lib()
         P, I, Lg, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
         L.tcb_page_plan.argtypes = [P, I, I, P, P, P, I, Lg, P, I, P, I, P, P, P, P, P, P, P]
-        L.tcb_kv_append.argtypes = [P, P, I, P, P, I, Lg, P, P]
+        L.tcb_kv_append.argtypes = [P, P, I, P, Lg, P, Lg, I, P, P]
         L.tcb_page_attn.argtypes = [P, P, I, I, I, P, Lg, P, Lg, P, P, P, I, Lg, I, I, F, I, I, P]
         L.tcb_prefix_attn.argtypes = [P, P, I, I, P, Lg, P, Lg, P, I, P, P, I, Lg, I, F, P]
         L.tcb_logits_penalize.argtypes = [P, P, P]
@@ -131,16 +131,16 @@ class Pages:
         self._dtype = k.dtype
 
     def append(self, k, v, slots, stream=None):
-        """tcb_kv_append: k and v [T, KV heads * head dim], rows of one stride
-        (views of the projection's rows do), to slots int64 [T]."""
+        """tcb_kv_append: k and v [T, KV heads * head dim] (float32, float16 or
+        bfloat16; parts of the projection's rows do), to slots int64 [T]."""
         T, n = k.shape
-        _need(k.dtype == v.dtype and k.shape == v.shape and k.stride() == v.stride() and k.is_cuda and v.is_cuda,
-              "k and v: two CUDA tensors of one shape, type and strides are wanted")
-        _need(n == self.kv_heads * self.head_dim and (n == 1 or k.stride(1) == 1), "k and v: [T, KV heads * head dim] is wanted")
+        _need(k.dtype is v.dtype and k.shape == v.shape and k.is_cuda and v.is_cuda, "k and v: two CUDA tensors of one shape and type are wanted")
+        (ldk, uk), (ldv, uv) = k.stride(), v.stride()
+        _need(n == self.kv_heads * self.head_dim and uk == 1 and uv == 1, "k and v: [T, KV heads * head dim] with dense rows is wanted")
         if k.dtype not in _TYPE:
             raise TcbError(2, "tcb_kv_append")
-        rc = _lib().tcb_kv_append(self.ctx.handle, self._ref, T, k.data_ptr(), v.data_ptr(), _TYPE[k.dtype],
-                                  k.stride(0) if T > 1 else n, _vec(slots, T, _I64, "slots"), _stream(self.ctx, stream))
+        rc = _lib().tcb_kv_append(self.ctx.handle, self._ref, T, k.data_ptr(), ldk if T > 1 else n, v.data_ptr(),
+                                  ldv if T > 1 else n, _TYPE[k.dtype], _vec(slots, T, _I64, "slots"), _stream(self.ctx, stream))
         self.ctx._check(rc, "tcb_kv_append")
 
     def _q(self, q, out):

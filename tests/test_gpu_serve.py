@@ -126,6 +126,8 @@ def test_append(ctx, xt, dt, layout, T_, KVH, hd, page, skew):
     wide = torch.randn(T_, 2 * KVH * hd + 8, device="cuda") * torch.logspace(-6, 4, T_, device="cuda")[:, None]
     wide = wide.to(xt)
     kr, vr = wide[:, skew:skew + KVH * hd], wide[:, KVH * hd + skew:2 * KVH * hd + skew]  # skew 1: rows off 16-byte alignment
+    if page == 64:
+        vr = vr.contiguous()  # rows of another stride
     slots = torch.randperm(n_pages * page, device="cuda")[:T_]
     if T_ > 4:
         slots[1] = -1

@@ -42,7 +42,7 @@ def prefix(ctx, kv=None, **kw):
 
 
 def append(ctx, kv=None, **kw):
-    d = dict(T=2, k=0x1000, v=0x2000, xdtype=T.F32, ldx=256, slots=0x100)
+    d = dict(T=2, k=0x1000, ldk=256, v=0x2000, ldv=256, xdtype=T.F32, slots=0x100)
     d.update(kw)
     return serve._lib().tcb_kv_append(ctx, ctypes.byref(pages() if kv is None else kv), *d.values(), None)
 
@@ -93,7 +93,7 @@ def test_prefix_attention(ctx, bad, code):
 
 
 @pytest.mark.parametrize("bad,code", [
-    (dict(T=-1), SHAPE), (dict(ldx=255), SHAPE), (dict(xdtype=T.Q4_K), DTYPE), (dict(k=0), NULL), (dict(slots=0), NULL),
+    (dict(T=-1), SHAPE), (dict(ldk=255), SHAPE), (dict(ldv=255), SHAPE), (dict(xdtype=T.Q4_K), DTYPE), (dict(k=0), NULL), (dict(slots=0), NULL),
     (dict(k=0x1002), ALIGN), (dict(slots=0x104), ALIGN), (dict(T=0), 0)])
 def test_append(ctx, bad, code):
     assert append(ctx, **bad) == code
