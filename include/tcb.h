@@ -404,8 +404,8 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H,
  * positions, one row each (row b of q and out is request b):
  *   out[b, h] = softmax over j < kv_len[b] of scale * q[b, h] . k[j], times v
  * with positions j < prefix_len read from the pages prefix[j / page] (device,
- * ceil(prefix_len / page) page numbers), once for all requests, and the
- * others from tables[b][j / page] as in tcb_page_attn (entries of whole
+ * ceil(prefix_len / page) page numbers), once for all requests where that is
+ * faster (long prefixes, many requests), and the others from tables[b][j / page] as in tcb_page_attn (entries of whole
  * prefix pages are not read).  kv_len[b] may be below prefix_len; 0 gives
  * zeros. */
 int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H,

@@ -45,8 +45,9 @@ struct RowsPlan {
 RowsPlan page_rows_plan(const PageAttnArgs &a);
 int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, void *scratch, cudaStream_t s);
 
-// Requests of one row (tcb_page_decode.cu).  With a.prefix set: the positions
-// from a.prefix_len on, joined with `parts` partial results as above.
+// Requests of one row (tcb_page_decode.cu).  With a.prefix set: its positions
+// from those pages, the others from the tables; or, with `parts` > 0, the
+// positions from a.prefix_len on (suffix), joined with partial results as above.
 struct DecodePlan {
   int nt, units, split;
   size_t o_bytes, bytes;  // scratch of the join across clusters
@@ -58,7 +59,7 @@ struct PrefixPartials {
   const float *o;
   const float2 *ml;
 };
-DecodePlan page_decode_plan(const PageAttnArgs &a);
+DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix);
 int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, const DecodePlan &pl, void *scratch, const PrefixPartials &x,
                        cudaStream_t s);
 

@@ -153,11 +153,18 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   }
   if (bad && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
   if (!live) return;  // every CTA of the cluster leaves
-  // visible: [lo, len) and [0, first); 16-position groups [0, ns) and [w0, w1)
-  int lo = a.window < 0 ? min(a.prefix_len, len) : (int)max(0l, (long)len - a.window);
-  int first = min(a.sinks, lo);
-  if (first == lo && first > 0) lo = first = 0;
-  const int ns = (first + 15) >> 4, w0 = max(lo >> 4, ns), w1 = lo < len ? max((len + 15) >> 4, w0) : w0;
+  // visible: [0, first) (the first positions, or a prefix read here) and
+  // [lo, len), first <= lo; in 16-position groups [0, ns) and [w0, w1)
+  int lo, first;
+  if (a.prefix) {
+    lo = min(a.prefix_len, len);
+    first = x.parts ? 0 : lo;
+  } else {
+    lo = a.window < 0 ? 0 : (int)max(0l, (long)len - a.window);
+    first = min(a.sinks, lo);
+    if (first == lo) lo = first = 0;
+  }
+  const int ns = (first + 15) >> 4, w0 = lo >> 4, w1 = lo < len ? (len + 15) >> 4 : w0;
   const int units = ns + w1 - w0;
   const int u0 = (int)((long)units * blockIdx.x / n_cta), u1 = (int)((long)units * (blockIdx.x + 1) / n_cta);
 
@@ -191,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   auto group_of = [&](int u) { return u < ns ? u : u - ns + w0; };
   auto page_of = [&](int u) {
     if (u >= u1) return 0;
-    const int pg = table[group_of(u) >> (a.page_shift - 4)];
+    const int at = group_of(u) >> (a.page_shift - 4), pg = u < ns && a.prefix ? a.prefix[at] : table[at];
     return pg >= 0 && pg < a.kv.n_pages ? pg : -1;
   };
   const int base = u0 + warp, n_it = base < u1 ? (u1 - base + kWarps - 1) / kWarps : 0;
@@ -230,6 +237,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   for (int i = 0; i < n_it; i++) {
     const bool here = ok;
     const int key0 = group_of(base + i * kWarps) << 4;
+    const bool early = base + i * kWarps < ns;
+    const int from = early ? 0 : lo, to = early ? first : len;
     float s[NT][4];
 #pragma unroll
     for (int x = 0; x < NT; x++) {
@@ -250,8 +259,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
       off = locate(i + 1, ok);
       load_k(off);
     }
-    const bool edge = !here || key0 + 16 > len || (key0 < lo && key0 + 16 > first);
-    auto sees = [&](int key) { return here && key < len && (key >= lo || key < first); };
+    const bool edge = !here || key0 < from || key0 + 16 > to;
+    auto sees = [&](int key) { return here && key >= from && key < to; };
     bool up = false;
 #pragma unroll
     for (int x = 0; x < NT; x++)
@@ -489,13 +498,13 @@ cudaError_t launch(const PageAttnArgs &a, const DecodePlan &pl, const Join &j, c
 
 }  // namespace pd
 
-DecodePlan page_decode_plan(const PageAttnArgs &a) {
+DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix) {
   DecodePlan pl{};
   const int G = a.H / a.kv.n_kv_heads;
   pl.nt = G <= 8 ? 1 : 2;
   const int q = 8 * pl.nt;
   long seen = a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
-  if (a.prefix) seen = std::max(0, a.max_len - a.prefix_len) + 16;
+  if (suffix) seen = std::max(0, a.max_len - a.prefix_len) + 16;
   const long groups = (seen + 15) / 16;  // of 16 positions, in the longest request
   const long units = (long)a.B * a.kv.n_kv_heads * ((G + q - 1) / q);
   pl.units = (int)units;

@@ -352,7 +352,7 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H, con
                       nullptr, 0, std::min(max_rows, T), max_len, scale * kLog2e, window, sinks, ctx->derr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (max_rows == 1) {
-    const tcb::DecodePlan pl = tcb::page_decode_plan(a);
+    const tcb::DecodePlan pl = tcb::page_decode_plan(a, false);
     if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
     return tcb::launch_page_decode(ctx, a, pl, ctx->ws, {}, s);
   }
@@ -375,14 +375,22 @@ int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const vo
   tcb::PageAttnArgs a{*kv, log2i(kv->page), B, B, H, q, ldq, out, ldo, nullptr, kv_len, tables, width, ldt,
                       prefix_len ? prefix : nullptr, prefix_len, 1, max_len, scale * kLog2e, -1, 0, ctx->derr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const tcb::DecodePlan dp = tcb::page_decode_plan(a);
+  // The prefix in a product of all requests' rows, or read by each request like
+  // its own positions (mostly from L2): the first costs about 10 us and 1.2 ns
+  // a position more, the second a quarter of a microsecond per MB.  With 8 KV
+  // heads of 128 and 4 query heads each, apart / read by each, in us: 4 requests
+  // behind 1024 positions 18.6 / 9.9, behind 4096 20.6 / 26.0; 16 behind 256 17.6 /
+  // 10.3, behind 1024 18.5 / 23.9; 64 behind 256 26.7 / 25.1, behind 4096 33.9 / 146
+  const double read = (double)B * prefix_len * kv->n_kv_heads * kv->head_dim * 4;
+  const bool apart = read > 40e6 + 4800. * prefix_len;
+  const tcb::DecodePlan dp = tcb::page_decode_plan(a, apart);
   tcb::RowsPlan rp{};
-  if (prefix_len) rp = tcb::page_rows_plan(a);
+  if (apart) rp = tcb::page_rows_plan(a);
   const size_t at = (rp.bytes + 255) / 256 * 256;
   if ((rc = tcb::ctx_ws(ctx, at + dp.bytes)) != TCB_OK) return rc;
   char *ws = static_cast<char *>(ctx->ws);
   tcb::PrefixPartials x{};
-  if (prefix_len) {
+  if (apart) {
     if ((rc = tcb::launch_page_rows(ctx, a, rp, ws, s)) != TCB_OK) return rc;
     x = {rp.split, reinterpret_cast<const float *>(ws), reinterpret_cast<const float2 *>(ws + rp.o_bytes)};
   }

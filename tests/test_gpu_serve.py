@@ -404,7 +404,10 @@ def test_attend_on_a_side_stream_and_in_a_graph(ctx):
 @pytest.mark.parametrize("B,P,H,KVH,hd,page,layout", [
     (1, 1, 4, 2, 128, 16, "heads"), (3, 15, 4, 1, 64, 16, "positions"), (5, 16, 8, 2, 128, 16, "both"), (9, 17, 6, 3, 64, 32, "heads"),
     (4, 300, 32, 8, 128, 64, "heads"), (33, 511, 16, 2, 128, 16, "positions"), (64, 130, 8, 8, 64, 256, "heads"), (40, 640, 32, 1, 128, 128, "both"),
-    (17, 0, 8, 2, 128, 16, "heads"), (7, 2100, 14, 2, 64, 16, "heads")])
+    (17, 0, 8, 2, 128, 16, "heads"), (7, 2100, 14, 2, 64, 16, "heads"),
+    # read once for all requests from here on
+    (64, 1111, 16, 8, 128, 16, "heads"), (61, 777, 32, 4, 128, 64, "positions"), (33, 2049, 24, 8, 64, 256, "both"), (5, 9000, 8, 2, 128, 32, "heads"),
+    (64, 4100, 20, 1, 128, 128, "heads"), (48, 900, 7, 7, 128, 16, "positions")])
 def test_attend_prefix(ctx, dtype, B, P, H, KVH, hd, page, layout):
     r = random.Random(P + B)
     lens = [P + r.choice([0, 1, 2, 15, 16, 17, 100, 200]) for _ in range(B)]
@@ -440,23 +443,25 @@ def test_attend_prefix(ctx, dtype, B, P, H, KVH, hd, page, layout):
             assert (out[b] == 0).all()
 
 
-def test_attend_prefix_nonfinite_tail_of_the_prefix(ctx):
+@pytest.mark.parametrize("P,B", [(100, 3), (2300, 63)])
+def test_attend_prefix_nonfinite_tail_of_the_prefix(ctx, P, B):
     """Requests shorter than the prefix do not see its later positions."""
-    P, page, hd = 100, 16, 128
-    k, v = pools(9, 1, page, hd, F16)
-    x = torch.randn(P, 1, hd, device="cuda").half()
+    page, hd, KVH = 16, 128, 1 if P == 100 else 2
+    n = -(-P // page)
+    k, v = pools(n + 2, KVH, page, hd, F16)
+    x = torch.randn(P, KVH, hd, device="cuda").half()
     y = x.clone()
     y[60:] = math.inf
-    put(k, list(range(7)), x, page)
-    put(v, list(range(7)), y, page)
-    q = torch.randn(3, 4, hd, device="cuda").half()
+    put(k, list(range(n)), x, page)
+    put(v, list(range(n)), y, page)
+    q = torch.randn(B, 4, hd, device="cuda").half()
     out = torch.empty_like(q)
-    lens = [60, 100, 31]
-    serve.Pages(ctx, k, v).attend_prefix(q, out, i32(list(range(7))), P, i32(lens), i32([[-1] * 7] * 3), P)
+    lens = [60, P, 31] + [P] * (B - 3)
+    serve.Pages(ctx, k, v).attend_prefix(q, out, i32(list(range(n))), P, i32(lens), i32([[-1] * n] * B), P)
     for b in (0, 2):
         want, mag = R.attention(q[b:b + 1].double(), x.double(), x.double(), [lens[b] - 1], 1 / math.sqrt(hd))
         assert ((out[b:b + 1].double() - want).abs() <= R.attention_bound(want, mag, P, F16)).all()
-    assert not torch.isfinite(out[1]).any()
+    assert not torch.isfinite(out[1]).any() and not torch.isfinite(out[3:]).any()
 
 
 def test_attend_prefix_device_findings(ctx):
@@ -464,6 +469,11 @@ def test_attend_prefix_device_findings(ctx):
     q = torch.randn(2, 2, 64, device="cuda").half()
     out = torch.empty_like(q)
     p = serve.Pages(ctx, k, v)
+    many = torch.randn(64, 2, 64, device="cuda").half()  # read once for all
+    pages = [0, 1, 2] * 1000
+    pages[1500] = 4
+    p.attend_prefix(many, torch.empty_like(many), i32(pages), 48000, i32([48000] * 64), i32([[-1] * 3000] * 64), 48000)
+    assert ctx.device_error(clear=True) == BOUNDS
     p.attend_prefix(q, out, i32([0, 99]), 32, i32([32, 32]), i32([[-1, -1, 2]] * 2), 40)
     assert ctx.device_error(clear=True) == BOUNDS
     p.attend_prefix(q, out, i32([0, 1]), 32, i32([33, 41]), i32([[-1, -1, 2]] * 2), 40)
