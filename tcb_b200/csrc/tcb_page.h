@@ -45,7 +45,7 @@ struct RowsPlan {
 RowsPlan page_rows_plan(const PageAttnArgs &a);
 int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, void *scratch, cudaStream_t s);
 
-// Requests of one row (tcb_page_decode.cu).  With a.prefix set: its positions
+// Row by row (tcb_page_decode.cu): every row reads the positions it sees.  With a.prefix set: its positions
 // from those pages, the others from the tables; or, with `parts` > 0, the
 // positions from a.prefix_len on (suffix), joined with partial results as above.
 struct DecodePlan {

@@ -1,7 +1,9 @@
-// tcb_page_decode.cu - attention over the paged cache for requests of one
-// row (a decode step; tcb_page_attn with max_rows 1).
+// tcb_page_decode.cu - attention over the paged cache row by row: decode steps
+// and few rows over few positions (tcb_page_attn), and batches behind a shared
+// prefix (tcb_prefix_attn: all of it, or the suffixes joined with partial results
+// of the prefix).
 //
-// Mathematics: per (request, KV head) the G = H / KVH query heads that share
+// Mathematics: per (row, KV head) the G = H / KVH query heads that share
 // the head are the 8 or 16 columns of two products on the tensor cores,
 //   S^T = K Q^T   (16 positions x queries, per 16 positions)
 //   O^T += V^T P^T (head elements x queries)
@@ -134,18 +136,20 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   __shared__ float xm[Q], xl[Q], xg[kMaxPrefixParts][Q];  // the prefix's partials: maximum, sum, weights
   const int G = a.H / a.kv.n_kv_heads, tiles = (G + Q - 1) / Q;
   const int kh = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * Q;  // first query head within the group
-  const int b = blockIdx.z, n_cta = gridDim.x;
+  const int b = blockIdx.z / a.max_rows, at = blockIdx.z - b * a.max_rows, n_cta = gridDim.x;  // row `at` of request b
   const int n_rank = j.ranks, c = blockIdx.x % n_rank, part = blockIdx.x / n_rank;  // rank in the cluster; cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  // the row of the request
+  // the row, and the positions up to its own
   int r = b, rows = 1;
+  bool bad = false;
   if (a.row_start) {
-    r = a.row_start[b];
-    rows = a.row_start[b + 1] - r;
+    const int r0 = min(max(a.row_start[b], 0), a.T);
+    rows = min(max(a.row_start[b + 1], r0), a.T) - r0;
+    r = r0 + at;
+    bad = rows > a.max_rows;
   }
-  bool bad = r < 0 || rows > 1;
-  const bool live = r >= 0 && r < a.T && rows >= 1;
+  const bool live = at < rows;
   int len = a.kv_len[b];
   if (len < 0 || len > a.max_len || len > (long)a.width << a.page_shift) {
     bad = true;
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   }
   if (bad && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
   if (!live) return;  // every CTA of the cluster leaves
+  len = max(len - rows + at + 1, 0);
   // visible: [0, first) (the first positions, or a prefix read here) and
   // [lo, len), first <= lo; in 16-position groups [0, ns) and [w0, w1)
   int lo, first;
@@ -481,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
 template <int DT, int HD, int NT>
 cudaError_t launch(const PageAttnArgs &a, const DecodePlan &pl, const Join &j, const PrefixPartials &x, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.split, pl.units / a.B, a.B);
+  cfg.gridDim = dim3(pl.split, pl.units / (a.B * a.max_rows), a.B * a.max_rows);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -506,7 +511,7 @@ DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix) {
   long seen = a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
   if (suffix) seen = std::max(0, a.max_len - a.prefix_len) + 16;
   const long groups = (seen + 15) / 16;  // of 16 positions, in the longest request
-  const long units = (long)a.B * a.kv.n_kv_heads * ((G + q - 1) / q);
+  const long units = (long)a.B * a.max_rows * a.kv.n_kv_heads * ((G + q - 1) / q);
   pl.units = (int)units;
   // CTAs per unit, doubled
   //  - while one wave of CTAs holds them (about 4 a SM) and a warp keeps 2 groups: one

@@ -351,7 +351,14 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H, con
   tcb::PageAttnArgs a{*kv, log2i(kv->page), B, T, H, q, ldq, out, ldo, row_start, kv_len, tables, width, ldt,
                       nullptr, 0, std::min(max_rows, T), max_len, scale * kLog2e, window, sinks, ctx->derr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (max_rows == 1) {
+  // Few rows over few positions go row by row too, each reading its positions
+  // again (mostly from L2), where that is at most 20 MB: with 8 KV heads of 128,
+  // row by row / by tiles in us: one request of 4 rows over 1024 positions 9.3 /
+  // 15.5, of 8 rows 18.2 / 15.4; 4 requests of 2 rows over 256 8.3 / 11.8, over 1024
+  // 18.4 / 15.5
+  const double seen = window < 0 ? max_len : std::min<double>(max_len, (double)window + sinks);
+  const double read = (double)B * a.max_rows * seen * kv->n_kv_heads * kv->head_dim * 4;
+  if (a.max_rows == 1 || (read <= 20e6 && (long)B * a.max_rows <= 65535)) {
     const tcb::DecodePlan pl = tcb::page_decode_plan(a, false);
     if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
     return tcb::launch_page_decode(ctx, a, pl, ctx->ws, {}, s);

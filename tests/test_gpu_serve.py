@@ -216,6 +216,21 @@ def test_attend_ragged_rows(ctx, dtype, window, sinks, H, KVH, hd, page, layout)
     check_rows(out, c, lens, rows, dtype, window, sinks, 1 / math.sqrt(hd), "rows")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (37, 0), (100, 17), (4, 64), (0, 5), (0, 0)])
+@pytest.mark.parametrize("H,KVH,hd,page,layout", [(8, 2, 128, 16, "heads"), (6, 6, 64, 64, "positions"), (16, 1, 128, 32, "both"),
+                                                   (28, 4, 64, 256, "heads"), (40, 2, 128, 128, "positions")])
+def test_attend_by_tiles(ctx, dtype, window, sinks, H, KVH, hd, page, layout):
+    """The same through the tiles of many rows: max_rows and max_len only bound
+    what the requests have, and bounds this large keep the rows together."""
+    lens = [1, 0, 3, 16, 33, 64, 150, 260, 300]
+    rows = [1, 2, 5, 16, 2, 30, 0, 129, 3]
+    c = attn_case(lens, rows, H, KVH, hd, page, dtype, layout, seed=H + hd + 2)
+    out = torch.full_like(c["q"], math.nan)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], 188, 70000, window=window, sinks=sinks)
+    check_rows(out, c, lens, rows, dtype, window, sinks, 1 / math.sqrt(hd), "tiles")
+
+
 @pytest.mark.parametrize("rows,n", [([1], 5000), ([1], 4097), ([2], 3000), ([200], 2100), ([517], 517), ([1030], 1500)])
 @pytest.mark.parametrize("dtype,H,KVH,hd", [(F16, 4, 1, 128), (BF16, 6, 2, 64)])
 def test_attend_longer(ctx, rows, n, dtype, H, KVH, hd):
@@ -252,9 +267,10 @@ def test_attend_growing_and_falling_scores(ctx):
             check_rows(out, c, [n, n], rows, BF16, None, 0, 1.0, "monotone scores")
 
 
+@pytest.mark.parametrize("most", [200, 1 << 20])  # row by row, by tiles
 @pytest.mark.parametrize("rows", [1, 3, 64])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_attend_nonfinite_where_nothing_looks(ctx, rows, bad):
+def test_attend_nonfinite_where_nothing_looks(ctx, rows, bad, most):
     """Non-finite K and V at cached positions outside the window of the last
     rows (and visible to none, or to the first rows only): rows that do not see
     them are unaffected; rows that see them are not finite."""
@@ -267,7 +283,8 @@ def test_attend_nonfinite_where_nothing_looks(ctx, rows, bad):
         for p in spots:
             c[name][c["tables"][0, p // page].item(), :, p % page] = bad
     out = torch.empty_like(c["q"])
-    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows, n, window=window, sinks=sinks)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows if most == n else most, most,
+                                            window=window, sinks=sinks)
     at = list(range(1 if rows > 1 else 0, rows))
     want, mag = R.attention(c["q"][at].double(), clean_k, clean_v, [n - rows + i for i in at], 1 / math.sqrt(hd), window, sinks)
     assert ((out[at].double() - want).abs() <= R.attention_bound(want, mag, n, F16)).all()
@@ -275,22 +292,23 @@ def test_attend_nonfinite_where_nothing_looks(ctx, rows, bad):
         assert torch.isnan(out[0]).all()
 
 
+@pytest.mark.parametrize("most", [100, 1 << 20])
 @pytest.mark.parametrize("rows", [2, 40])
-def test_attend_nonfinite_after_a_row(ctx, rows):
+def test_attend_nonfinite_after_a_row(ctx, rows, most):
     """A later position's V is infinite: rows before it do not see it."""
     n, hd = 100, 64
     c = attn_case([n], [rows], 2, 2, hd, 16, BF16, seed=rows)
     c["v"][c["tables"][0, (n - 1) // 16].item(), :, (n - 1) % 16] = math.inf
     out = torch.empty_like(c["q"])
-    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows, n)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows, most)
     at = list(range(rows - 1))
     want, mag = R.attention(c["q"][at].double(), *c["kv"][0], [n - rows + i for i in at], 1 / math.sqrt(hd))
     assert ((out[at].double() - want).abs() <= R.attention_bound(want, mag, n, BF16)).all()
     assert not torch.isfinite(out[rows - 1]).any()
 
 
-@pytest.mark.parametrize("rows", [1, 20])
-def test_attend_strided_rows_and_untouched_ones(ctx, rows):
+@pytest.mark.parametrize("rows,most", [(1, 90), (20, 90), (20, 1 << 20)])
+def test_attend_strided_rows_and_untouched_ones(ctx, rows, most):
     """q as a part of wider rows, out likewise; rows outside every request keep what they hold."""
     lens, m = [50, 90], [rows, rows]
     c = attn_case(lens, m, 4, 2, 64, 32, F16, seed=rows)
@@ -299,20 +317,20 @@ def test_attend_strided_rows_and_untouched_ones(ctx, rows):
     q[:2 * rows] = c["q"]
     res = torch.full((2 * rows + 3, 6 * 64), 9.0, dtype=F16, device="cuda")
     out = res.view(-1, 6, 64)[:, 1:5]
-    serve.Pages(ctx, c["k"], c["v"]).attend(q, out, c["row_start"], c["kv_len"], c["tables"], rows, 90)
+    serve.Pages(ctx, c["k"], c["v"]).attend(q, out, c["row_start"], c["kv_len"], c["tables"], rows, most)
     check_rows(out, c, lens, m, F16, None, 0, 1 / 8, "strided")
     assert (out[2 * rows:] == 9).all() and (res.view(-1, 6, 64)[:, 0] == 9).all() and (res.view(-1, 6, 64)[:, 5] == 9).all()
 
 
-@pytest.mark.parametrize("rows", [1, 24])
-def test_attend_device_findings(ctx, rows):
+@pytest.mark.parametrize("rows,most", [(1, 64), (24, 64), (24, 1 << 20)])
+def test_attend_device_findings(ctx, rows, most):
     """A page outside the pools, a length past max_len or the table, and more
     rows than max_rows are reported, and the other requests are right."""
     lens, m = [40, 64, 33], [rows, rows, rows]
     c = attn_case(lens, m, 4, 2, 128, 16, BF16, seed=rows)
     p = serve.Pages(ctx, c["k"], c["v"])
 
-    def go(tables=None, kv_len=None, row_start=None, max_rows=rows, max_len=64):
+    def go(tables=None, kv_len=None, row_start=None, max_rows=rows, max_len=most):
         out = torch.zeros_like(c["q"])
         p.attend(c["q"], out, c["row_start"] if row_start is None else row_start, c["kv_len"] if kv_len is None else kv_len,
                  c["tables"] if tables is None else tables, max_rows, max_len)
@@ -326,7 +344,7 @@ def test_attend_device_findings(ctx, rows):
         for b in (0, 2):
             sub = {**c, "q": c["q"][b * rows:(b + 1) * rows], "kv": [c["kv"][b]], "start": [0]}
             check_rows(out[b * rows:(b + 1) * rows], sub, [lens[b]], [rows], BF16, None, 0, 1 / math.sqrt(128), "neighbour")
-    for n in (65, 2 ** 31 - 1, -1):
+    for n in (65 if most == 64 else 16 * c["tables"].shape[1] + 1, 2 ** 31 - 1, -1):
         out = go(kv_len=i32([40, n, 33]))
         assert ctx.device_error(clear=True) == BOUNDS
         sub = {**c, "q": c["q"][:rows], "kv": [c["kv"][0]], "start": [0]}
@@ -340,8 +358,8 @@ def test_attend_device_findings(ctx, rows):
         assert ctx.device_error(clear=True) == BOUNDS
 
 
-@pytest.mark.parametrize("rows", [1, 70])
-def test_attend_offsets_past_32_bits(ctx, rows):
+@pytest.mark.parametrize("rows,most", [(1, 200), (3, 200), (70, 1 << 20)])
+def test_attend_offsets_past_32_bits(ctx, rows, most):
     """Pages whose elements lie past 2^31 and 2^32 of the pool (K and V in one
     array; only the pages in use are written)."""
     KVH, page, hd = 2, 64, 128
@@ -357,7 +375,7 @@ def test_attend_offsets_past_32_bits(ctx, rows):
     c = dict(q=torch.randn(rows, 4, hd, device="cuda").to(BF16), kv=[(x.double(), x.double())], start=[0])
     out = torch.empty_like(c["q"])
     p = serve.Pages(ctx, pool, pool)
-    p.attend(c["q"], out, i32([0, rows]), i32([n]), i32([table]), rows, n)
+    p.attend(c["q"], out, i32([0, rows]), i32([n]), i32([table]), rows, most)
     check_rows(out, c, [n], [rows], BF16, None, 0, 1 / math.sqrt(hd), "far pages")
     # and the append finds them
     y = torch.randn(1, KVH * hd, device="cuda")
@@ -365,15 +383,15 @@ def test_attend_offsets_past_32_bits(ctx, rows):
     assert torch.equal(pool[n_pages - 1, :, 5], y.view(KVH, hd).to(BF16))
 
 
-@pytest.mark.parametrize("rows", [1, 33])
-def test_attend_again_is_the_same_bits(ctx, rows):
+@pytest.mark.parametrize("rows,most", [(1, 1000), (33, 1000), (33, 1 << 20)])
+def test_attend_again_is_the_same_bits(ctx, rows, most):
     lens = [500, 3, 64, 1000]
     m = [min(rows, n) for n in lens]
     c = attn_case(lens, m, 8, 2, 128, 16, F16, seed=1)
     p, outs = serve.Pages(ctx, c["k"], c["v"]), []
     for _ in range(3):
         out = torch.full_like(c["q"], math.nan)
-        p.attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows, 1000)
+        p.attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], rows, most)
         outs.append(out)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
