@@ -42,7 +42,7 @@ struct Pick {
 
 // four elements from index i on; VEC: aligned to the four
 template <int DT, bool VEC>
-__device__ __forceinline__ float4 load4(const void *p, long i, int n) {
+__device__ __forceinline__ float4 load4(const void *p, int i, int n) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if constexpr (VEC) {
     if (n >= 4) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ float4 load4(const void *p, long i, int n) {
   return v;
 }
 template <int DT, bool VEC>
-__device__ __forceinline__ void store4(void *p, long i, int n, const float (&v)[4]) {
+__device__ __forceinline__ void store4(void *p, int i, int n, const float (&v)[4]) {
   if constexpr (VEC) {
     if (n >= 4) {
       if constexpr (DT == TCB_F32) {
@@ -88,12 +88,15 @@ __global__ void __launch_bounds__(kMaxThreads, 2) k_penalize(const __grid_consta
   const int b = blockIdx.y, t0 = blockIdx.x * tile, n = min(tile, a.V - t0);
   const bool counted = a.history, biased = a.n_bias > 0;
 
+  const char *in_row = static_cast<const char *>(a.logits) + b * a.ld * (XT == TCB_F32 ? 4 : 2);
+  char *out_row = static_cast<char *>(a.out) + b * a.ldo * (OT == TCB_F32 ? 4 : 2);
+
   // everything that is read first is asked for before anything is waited for
   float4 x[kPer / 4];
 #pragma unroll
   for (int u = 0; u < kPer / 4; u++) {
     const int i = 4 * (u * nt + tid);
-    x[u] = load4<XT, VEC>(a.logits, b * a.ld + t0 + i, n - i);
+    x[u] = load4<XT, VEC>(in_row, t0 + i, n - i);
   }
   const int total = a.history ? min(max(a.total_len[b], 0), a.hist_width) : 0;
   const int prompt = a.history && a.prompt_len ? a.prompt_len[b] : 0;
@@ -123,7 +126,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) k_penalize(const __grid_consta
 #pragma unroll
   for (int u = 0; u < kPer / 4; u++) {
     const int i = 4 * (u * nt + tid);
-    word[u] = mask && i < n ? mask[(t0 + i) >> 5] >> ((t0 + i) & 31) : 0xFu;
+    const uint32_t in = (1u << min(max(n - i, 0), 4)) - 1u;  // tokens of the four that are in the row
+    word[u] = mask && i < n ? mask[(t0 + i) >> 5] >> ((t0 + i) & 31) & in : in;
   }
   if (tid == 0) best_s = 0;
   for (int i = tid; i < (biased ? 2 : counted ? 1 : 0) * tile / 4; i += nt) reinterpret_cast<uint4 *>(sh)[i] = make_uint4(0, 0, 0, 0);
@@ -182,14 +186,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) k_penalize(const __grid_consta
     }
     auto last = [&](float &v, int e) {
       if (!(word[u] >> e & 1)) v = -INFINITY;
-      if (v > best && i + e < n) best = v, best_t = t0 + i + e;
+      if (v > best) best = v, best_t = t0 + i + e;
     };
     last(x[u].x, 0);
     last(x[u].y, 1);
     last(x[u].z, 2);
     last(x[u].w, 3);
     const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-    store4<OT, VEC>(a.out, b * a.ldo + t0 + i, n - i, v);
+    store4<OT, VEC>(out_row, t0 + i, n - i, v);
   }
   if (a.token) {
     // the warp's largest value (in its order-preserving form; -0 and +0 are equal), then its lowest token
