@@ -12,6 +12,8 @@ Names follow TR's tensor.Backend quant branch:
   qembed      Backend.Embedding with quantized w (tensor/limits.go:15-45)
   quant_upload / quant_download   FromRaw / ToRaw (gpu/typed.go:24-55)
   quant_zero  QuantZeroRaw on the device (tensor/quant.go:416-427)
+The decoder engine is in tcb_b200.llama; the paged cache, its attention and the
+logits' penalties (no counterpart in TR) are in tcb_b200.serve.
 """
 from __future__ import annotations
 
