@@ -1,20 +1,25 @@
-"""Build libtcb.so (the sm_100a kernels + C ABI) in-tree with nvcc.
+"""Build libtcb.so (the sm_100a kernels + C ABI) in-tree with nvcc, and
+_tcb_torch.so (its serving entry points for torch tensors) with g++.
 
     python -m tcb_b200.build          # or tcb_b200.build.build()
 
-The library lands next to this file (tcb_b200/libtcb.so) so it travels
-with the source tree; nothing is installed into site-packages.
+The libraries land next to this file (tcb_b200/libtcb.so, _tcb_torch.so) so they
+travel with the source tree; nothing is installed into site-packages.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtcb.so")
+TORCH_LIB = os.path.join(HERE, "_tcb_torch.so")
+CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -42,6 +47,15 @@ def build(verbose: bool = False, force: bool = False) -> str:
         objs.append(o)
         if force or _stale([o], [s] + headers):
             cmds.append([NVCC, *ARCH, *FLAGS, "-c", s, "-o", o])
+
+    torch_src = os.path.join(CSRC, "tcb_torch.cpp")
+    if force or _stale([TORCH_LIB], [torch_src, headers[-1]]):
+        t = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+        cmds.append([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
+                     "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(t, "include"), "-isystem",
+                     os.path.join(t, "include", "torch", "csrc", "api", "include"), "-isystem", "/usr/local/cuda/include",
+                     torch_src, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+                     "-ltorch_python"])
 
     def compile_one(cmd):
         if verbose:

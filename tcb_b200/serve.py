@@ -1,5 +1,7 @@
 """Serving operators over a paged K/V cache (include/tcb.h, tcb_page_* and
-tcb_logits_penalize): a thin ctypes view for torch CUDA tensors.
+tcb_logits_penalize): a thin view for torch CUDA tensors (the checks and the
+call itself are in tcb_b200/csrc/tcb_torch.cpp; the C structures and argument
+types are here).
 
 One step of a batch of requests:
   plan(...)             pages, row offsets, slots and positions of the step
@@ -17,14 +19,13 @@ Context.device_error().
 from __future__ import annotations
 
 import ctypes
-import math
+import os
 
 import torch
 
-from . import BF16, F16, F32, TcbError, lib
+from . import BF16, F16, HERE, TcbError, lib
 
-_TYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-_I32, _I64 = torch.int32, torch.int64
+_TYPE = {torch.float16: F16, torch.bfloat16: BF16}
 
 
 class _KvPages(ctypes.Structure):
@@ -46,13 +47,6 @@ class _LogitsArgs(ctypes.Structure):
                 ("mask_row", ctypes.c_void_p)]
 
 
-def _stream(ctx, stream) -> int:
-    """The handle of `stream`, or of the current stream of the context's device."""
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(ctx.device)
-    return stream if isinstance(stream, int) else stream.cuda_stream
-
-
 _bound = None
 
 
@@ -70,26 +64,29 @@ def _lib():
     return _bound
 
 
+_torch_view = None
+
+
+def _view():
+    """The module _tcb_torch (tcb_b200/csrc/tcb_torch.cpp), bound to the loaded
+    library.  No fallback: a missing module raises."""
+    global _torch_view
+    if _torch_view is None:
+        path = os.path.join(HERE, "_tcb_torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing; build it with `python -m tcb_b200.build`")
+        from . import _tcb_torch as m
+
+        L = _lib()
+        m.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (L.tcb_page_plan, L.tcb_kv_append, L.tcb_page_attn,
+                                                                L.tcb_prefix_attn, L.tcb_logits_penalize)))
+        _torch_view = m
+    return _torch_view
+
+
 def _need(ok: bool, what: str):
     if not ok:
         raise ValueError(what)
-
-
-def _vec(t, n: int, dtype, name: str) -> int:
-    """Address of a contiguous device vector of at least n elements."""
-    if t.dtype is not dtype or not t.is_cuda or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous {dtype} CUDA vector of at least {n} elements is wanted")
-    return t.data_ptr()
-
-
-def _rows(t, dtype, name: str):
-    """(address, width, row stride) of a 2-D device tensor with dense rows."""
-    if t.dtype is not dtype or not t.is_cuda or t.dim() != 2:
-        raise ValueError(f"{name}: a 2-D {dtype} CUDA tensor with dense rows is wanted")
-    (n, width), (ld, unit) = t.shape, t.stride()
-    if width > 1 and unit != 1:
-        raise ValueError(f"{name}: a 2-D {dtype} CUDA tensor with dense rows is wanted")
-    return t.data_ptr(), width, ld if n > 1 else width
 
 
 def plan(ctx, page, cached, fresh, tables, free, n_free, row_start, kv_len, slots, positions, balance, taken=None,
@@ -99,16 +96,10 @@ def plan(ctx, page, cached, fresh, tables, free, n_free, row_start, kv_len, slot
     first n_free[0] are free; written: row_start int32 [B + 1], kv_len int32
     [B], slots int64 and positions int32 [rows], balance int32 [1] (the free
     pages left, below 0 the shortage), taken int32 [1] or None (pages taken)."""
-    B, rows = cached.shape[0], slots.shape[0]
-    tp, width, ldt = _rows(tables, _I32, "tables")
-    _need(tables.shape[0] >= B, "tables: a row per request is wanted")
-    rc = _lib().tcb_page_plan(ctx.handle, B, page, _vec(cached, B, _I32, "cached"), _vec(fresh, B, _I32, "fresh"), tp,
-                              width, ldt, _vec(free, 0, _I32, "free"), free.shape[0], _vec(n_free, 1, _I32, "n_free"),
-                              rows, _vec(row_start, B + 1, _I32, "row_start"), _vec(kv_len, B, _I32, "kv_len"),
-                              _vec(slots, 0, _I64, "slots"), _vec(positions, rows, _I32, "positions"),
-                              _vec(balance, 1, _I32, "balance"),
-                              0 if taken is None else _vec(taken, 1, _I32, "taken"), _stream(ctx, stream))
-    ctx._check(rc, "tcb_page_plan")
+    rc = _view().plan(ctx.handle.value, ctx.device, page, cached, fresh, tables, free, n_free, row_start, kv_len, slots,
+                      positions, balance, taken, stream)
+    if rc:
+        ctx._check(rc, "tcb_page_plan")
 
 
 class Pages:
@@ -127,61 +118,35 @@ class Pages:
         n_pages, self.kv_heads, self.page, self.head_dim = k.shape
         self._kv = _KvPages(k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], n_pages, self.page, self.kv_heads,
                             self.head_dim, k.stride(0), k.stride(1), k.stride(2))
-        self._ref = ctypes.byref(self._kv)
-        self._dtype = k.dtype
+        self._at = ctypes.addressof(self._kv)
+        _need(k.device.index == ctx.device, "k and v: tensors of the context's device are wanted")
 
     def append(self, k, v, slots, stream=None):
         """tcb_kv_append: k and v [T, KV heads * head dim] (float32, float16 or
         bfloat16; parts of the projection's rows do), to slots int64 [T]."""
-        T, n = k.shape
-        _need(k.dtype is v.dtype and k.shape == v.shape and k.is_cuda and v.is_cuda, "k and v: two CUDA tensors of one shape and type are wanted")
-        (ldk, uk), (ldv, uv) = k.stride(), v.stride()
-        _need(n == self.kv_heads * self.head_dim and uk == 1 and uv == 1, "k and v: [T, KV heads * head dim] with dense rows is wanted")
-        if k.dtype not in _TYPE:
-            raise TcbError(2, "tcb_kv_append")
-        rc = _lib().tcb_kv_append(self.ctx.handle, self._ref, T, k.data_ptr(), ldk if T > 1 else n, v.data_ptr(),
-                                  ldv if T > 1 else n, _TYPE[k.dtype], _vec(slots, T, _I64, "slots"), _stream(self.ctx, stream))
-        self.ctx._check(rc, "tcb_kv_append")
-
-    def _q(self, q, out):
-        if q.dtype != self._dtype or out.dtype != self._dtype:
-            raise TcbError(2, "q and out are of the cache's type")
-        _need(q.dim() == 3 and q.shape == out.shape and q.is_cuda and out.is_cuda, "q and out: [T, H, head dim] CUDA tensors are wanted")
-        T, H, hd = q.shape
-        _need(hd == self.head_dim, "q and out: the cache's head dim is wanted")
-        for t in (q, out):
-            _need(t.stride(2) == 1 and (H == 1 or t.stride(1) == hd), "q and out: dense heads are wanted")
-        return T, H, q.data_ptr(), q.stride(0) if T > 1 else H * hd, out.data_ptr(), out.stride(0) if T > 1 else H * hd
+        rc = _view().append(self.ctx.handle.value, self.ctx.device, self._at, k, v, slots, stream)
+        if rc:
+            self.ctx._check(rc, "tcb_kv_append")
 
     def attend(self, q, out, row_start, kv_len, tables, max_rows, max_len, scale=None, window=None, sinks=0, stream=None):
         """tcb_page_attn: q and out [T, H, head dim] in the cache's type;
         row_start int32 [B + 1], kv_len int32 [B], tables int32 [B, width];
         max_rows and max_len bound a request's rows and length; scale None is
         1 / sqrt(head dim), window None sees every earlier position."""
-        T, H, qp, ldq, op, ldo = self._q(q, out)
-        B = kv_len.shape[0]
-        tp, width, ldt = _rows(tables, _I32, "tables")
-        _need(tables.shape[0] >= B, "tables: a row per request is wanted")
-        _need(window is None or window >= 0, "window: None or a whole number from 0 is wanted")
-        rc = _lib().tcb_page_attn(self.ctx.handle, self._ref, B, T, H, qp, ldq, op, ldo,
-                                  _vec(row_start, B + 1, _I32, "row_start"), _vec(kv_len, B, _I32, "kv_len"), tp, width,
-                                  ldt, max_rows, max_len, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-                                  -1 if window is None else window, sinks, _stream(self.ctx, stream))
-        self.ctx._check(rc, "tcb_page_attn")
+        rc = _view().attend(self.ctx.handle.value, self.ctx.device, self._at, q, out, row_start, kv_len, tables, max_rows,
+                            max_len, scale, window, sinks, stream)
+        if rc:
+            self.ctx._check(rc, "tcb_page_attn")
         return out
 
     def attend_prefix(self, q, out, prefix, prefix_len, kv_len, tables, max_len, scale=None, stream=None):
         """tcb_prefix_attn: row b of q and out [B, H, head dim] is request b;
         prefix int32, the pages of the shared first prefix_len positions;
         kv_len int32 [B] counts them; tables int32 [B, width] as in attend."""
-        T, H, qp, ldq, op, ldo = self._q(q, out)
-        tp, width, ldt = _rows(tables, _I32, "tables")
-        _need(tables.shape[0] >= T, "tables: a row per request is wanted")
-        rc = _lib().tcb_prefix_attn(self.ctx.handle, self._ref, T, H, qp, ldq, op, ldo,
-                                    _vec(prefix, -(-prefix_len // self.page), _I32, "prefix"), prefix_len,
-                                    _vec(kv_len, T, _I32, "kv_len"), tp, width, ldt, max_len,
-                                    1.0 / math.sqrt(self.head_dim) if scale is None else scale, _stream(self.ctx, stream))
-        self.ctx._check(rc, "tcb_prefix_attn")
+        rc = _view().attend_prefix(self.ctx.handle.value, self.ctx.device, self._at, q, out, prefix, prefix_len, kv_len,
+                                   tables, max_len, scale, stream)
+        if rc:
+            self.ctx._check(rc, "tcb_prefix_attn")
         return out
 
 
@@ -192,37 +157,8 @@ def penalize(ctx, logits, out, token=None, history=None, prompt_len=None, total_
     width] with prompt_len and total_len int32 [B]; repetition, frequency and
     presence float32 [B]; bias_ids int32 and bias float32 [B, n]; mask int32
     [masks, ceil(V / 32)], mask_row int32 [B]."""
-    _need(logits.dim() == 2 and logits.shape == out.shape and logits.is_cuda and out.is_cuda, "logits and out: two [B, V] CUDA tensors are wanted")
-    B, V = logits.shape
-    for t in (logits, out):
-        if t.dtype not in _TYPE:
-            raise TcbError(2, "tcb_logits_penalize")
-        _need(V <= 1 or t.stride(1) == 1, "logits and out: dense rows are wanted")
-    f32 = torch.float32
-    hp = width = ldh = 0
-    if history is not None:
-        hp, width, ldh = _rows(history, _I64, "history")
-        _need(history.shape[0] >= B and total_len is not None, "history: a row per sequence and total_len are wanted")
-    ip = vp = nb = ldb = 0
-    if bias_ids is not None:
-        ip, nb, ldb = _rows(bias_ids, _I32, "bias_ids")
-        vp, nv, ldv = _rows(bias, f32, "bias")
-        _need(nv == nb and ldv == ldb and bias_ids.shape[0] >= B and bias.shape[0] >= B, "bias_ids and bias: two tensors of one shape and stride are wanted")
-    mp = nm = ldm = 0
-    if mask is not None:
-        mp, words, ldm = _rows(mask, _I32, "mask")
-        nm = mask.shape[0]
-        _need(words >= -(-V // 32) and (mask_row is not None or nm >= B), "mask: ceil(V / 32) words in a row, and a row per sequence or mask_row, are wanted")
-    a = _LogitsArgs(B, V, logits.data_ptr(), _TYPE[logits.dtype], logits.stride(0) if B > 1 else V,
-                    out.data_ptr(), _TYPE[out.dtype], out.stride(0) if B > 1 else V,
-                    _vec(token, B, _I64, "token") if token is not None else 0, hp, width, ldh,
-                    _vec(prompt_len, B, _I32, "prompt_len") if prompt_len is not None else 0,
-                    _vec(total_len, B, _I32, "total_len") if total_len is not None else 0,
-                    _vec(repetition, B, f32, "repetition") if repetition is not None else 0,
-                    _vec(frequency, B, f32, "frequency") if frequency is not None else 0,
-                    _vec(presence, B, f32, "presence") if presence is not None else 0,
-                    ip, vp, nb, ldb, mp, nm, ldm,
-                    _vec(mask_row, B, _I32, "mask_row") if mask_row is not None else 0)
-    rc = _lib().tcb_logits_penalize(ctx.handle, ctypes.byref(a), _stream(ctx, stream))
-    ctx._check(rc, "tcb_logits_penalize")
+    rc = _view().penalize(ctx.handle.value, ctx.device, logits, out, token, history, prompt_len, total_len, repetition,
+                          frequency, presence, bias_ids, bias, mask, mask_row, stream)
+    if rc:
+        ctx._check(rc, "tcb_logits_penalize")
     return out

@@ -84,6 +84,37 @@ def test_plan_of_nothing(ctx):
     assert left.item() == 2
 
 
+def test_tensors_that_are_not_what_is_wanted(ctx):
+    """Refused before anything is launched: types, sizes, strides, places."""
+    k, v = pools(4, 2, 16, 64, F16, fill=0.0)
+    p = serve.Pages(ctx, k, v)
+    q, rs, kl, t = torch.zeros(2, 4, 64, device="cuda", dtype=F16), i32([0, 1, 2]), i32([3, 4]), i32([[0], [1]])
+    x, s = torch.zeros(2, 128, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    lg, f = torch.zeros(2, 40, device="cuda"), torch.zeros(2, device="cuda")
+    i = i32([0, 0, 0])
+    refused = [lambda: p.attend(q, q, rs.long(), kl, t, 1, 16), lambda: p.attend(q, q, rs[:2], kl, t, 1, 16), lambda: p.attend(q, q, rs, kl.cpu(), t, 1, 16),
+               lambda: p.attend(q, q[:1], rs, kl, t, 1, 16), lambda: p.attend(q[..., :32], q[..., :32], rs, kl, t, 1, 16), lambda: p.attend(q, q, rs, kl, t[:1], 1, 16),
+               lambda: p.attend(q.transpose(0, 1), q.transpose(0, 1), rs, kl, t, 1, 16), lambda: p.attend(q, q, rs, kl, t, 1, 16, window=-2), lambda: p.attend(q, q, rs, kl, t, 2 ** 40, 16),
+               lambda: p.attend_prefix(q, q, i, 100, kl, t, 16), lambda: p.attend_prefix(q, q, i, -1, kl, t, 16), lambda: p.attend_prefix(q, q, i, 16, kl[:1], t, 16),
+               lambda: p.append(x, x[:1], s), lambda: p.append(x[:, :64], x[:, :64], s), lambda: p.append(x, x, s[:1]), lambda: p.append(x, x, s.int()), lambda: p.append(x.t(), x.t(), s),
+               lambda: serve.plan(ctx, 16, i, i[:2], t, i, i, i, i, s, i, i), lambda: serve.plan(ctx, 16, i[:2], i[:2], t, i, i, i[:2], i, s, i, i),
+               lambda: serve.plan(ctx, 16, i[:2], i[:2], t, i, i, i, i, s, i[:1], i), lambda: serve.plan(ctx, 16, i[:2], i[:2], t, i, i, i, i, s, i, None),
+               lambda: serve.penalize(ctx, lg, lg[:, :39]), lambda: serve.penalize(ctx, lg, lg, token=i), lambda: serve.penalize(ctx, lg, lg, history=torch.zeros(2, 3, dtype=torch.int64, device="cuda")),
+               lambda: serve.penalize(ctx, lg, lg, repetition=f[:1]), lambda: serve.penalize(ctx, lg, lg, bias_ids=i32([[1], [2]]), bias=f), lambda: serve.penalize(ctx, lg, lg, mask=i32([[1], [1]])),
+               lambda: serve.penalize(ctx, lg, lg, mask=i32([[1, 1]])), lambda: serve.penalize(ctx, lg, lg, repetition=[1.0, 1.0])]
+    for n, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {n} was taken")
+    for call in (lambda: p.attend(q.bfloat16(), q.bfloat16(), rs, kl, t, 1, 16), lambda: p.append(x.double(), x.double(), s), lambda: serve.penalize(ctx, lg.double(), lg),
+                 lambda: serve.Pages(ctx, k.float(), v.float())):
+        with pytest.raises(T.TcbError) as e:
+            call()
+        assert e.value.code == 2  # TCB_ERR_DTYPE
+    with pytest.raises(TypeError):
+        p.attend(q, q, rs, kl, t, "1", 16)
+
+
 # ------------------------------------------------------------ pools
 
 def pools(n_pages, KVH, page, hd, dtype, layout="heads", fill=math.nan):

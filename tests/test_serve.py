@@ -1,6 +1,7 @@
 """Refusals of the serving operators' C entry points and Python view, and the
 plan's reference, without a GPU."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -120,17 +121,16 @@ def test_logits(ctx, bad, code):
     assert logits(ctx, **bad) == code
 
 
-def test_python_view_refuses_host_tensors_and_types():
+def test_python_view_refuses_host_tensors(ctx):
+    c = types.SimpleNamespace(handle=ctypes.c_void_p(ctypes.addressof(ctx)), device=0)
     k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
-    with pytest.raises(ValueError):
-        serve.Pages(None, k, k)
-    with pytest.raises(ValueError):
-        serve.Pages(None, k, k[:2])
-    with pytest.raises(ValueError):
-        serve.penalize(None, torch.zeros(2, 8), torch.zeros(2, 8))
     i = torch.zeros(2, dtype=torch.int32)
-    with pytest.raises(ValueError):
-        serve.plan(None, 16, i, i, i.view(2, 1), i, i, i, i, i.long(), i, i)
+    for call in (lambda: serve.Pages(c, k, k), lambda: serve.Pages(c, k, k[:2]), lambda: serve.penalize(c, torch.zeros(2, 8), torch.zeros(2, 8)),
+                 lambda: serve.plan(c, 16, i, i, i.view(2, 1), i, i, i, i, i.long(), i, i), lambda: serve.plan(c, 16, None, i, i, i, i, i, i, i, i, i)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        serve._view().plan(0)
 
 
 def test_plan_reference():
