@@ -25,6 +25,8 @@
 #include "../../include/tcb.h"
 #include "tcb_common.cuh"
 #include "tcb_ctx.h"
+#include "tcb_mv_ptx.cuh"
+#include "tcb_page.h"
 
 namespace {
 
@@ -86,6 +88,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) k_penalize(const __grid_consta
   uint32_t *entry = sh + tile;  // [tile] 1 + last bias entry, 0: none (only with biases)
   __shared__ unsigned long long best_s;
   const int b = blockIdx.y, t0 = blockIdx.x * tile, n = min(tile, a.V - t0);
+  mv::pdl_wait();
   const bool counted = a.history, biased = a.n_bias > 0;
 
   const char *in_row = static_cast<const char *>(a.logits) + b * a.ld * (XT == TCB_F32 ? 4 : 2);
@@ -195,6 +198,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) k_penalize(const __grid_consta
     const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
     store4<OT, VEC>(out_row, t0 + i, n - i, v);
   }
+  mv::pdl_launch_dependents();  // here, not at the start: CTAs of the next kernel would wait in the room of this one's
   if (a.token) {
     // the warp's largest value (in its order-preserving form; -0 and +0 are equal), then its lowest token
     const uint32_t f = f_bits(best + 0.f), key = best_t < 0 ? 0u : f & 0x80000000u ? ~f : f | 0x80000000u;
@@ -228,8 +232,7 @@ cudaError_t launch(const tcb_logits_args &a, int threads, Pick *picks, int *derr
       return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     }();
     if (attr != cudaSuccess) return attr;
-    kernel<<<grid, threads, smem, s>>>(a, picks, derr);
-    return cudaGetLastError();
+    return launch_serve(kernel, grid, threads, smem, 1, s, a, picks, derr);
   };
   return vec ? go(k_penalize<XT, OT, true>) : go(k_penalize<XT, OT, false>);
 }

@@ -10,6 +10,30 @@
 
 namespace tcb {
 
+// Launch of a serving kernel (clusters of `cluster` CTAs along x): its CTAs may
+// be placed while the last kernel of the stream ends, so every one of them
+// waits for that kernel (mv::pdl_wait) before it touches memory, and lets the
+// next kernel do the same (mv::pdl_launch_dependents).  Between the small
+// kernels of a step this hides most of a launch.
+template <class... Params, class... Args>
+inline cudaError_t launch_serve(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s,
+                                const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // attention over the pages (tcb_page_attn, tcb_prefix_attn), arguments checked
 struct PageAttnArgs {
   tcb_kv_pages kv;
@@ -49,7 +73,7 @@ int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, vo
 // from those pages, the others from the tables; or, with `parts` > 0, the
 // positions from a.prefix_len on (suffix), joined with partial results as above.
 struct DecodePlan {
-  int nt, units, split;
+  int nt, units, split, warps;
   size_t o_bytes, bytes;  // scratch of the join across clusters
   size_t counters;        // bytes of zeroed counters
 };

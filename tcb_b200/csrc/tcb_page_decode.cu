@@ -48,8 +48,6 @@
 namespace tcb {
 namespace pd {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
 constexpr float kSlack = 8.f;
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 
@@ -73,7 +71,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// CTAs per SM that leave a thread the registers it needs without spills (168
+// CTAs of 4 warps per SM that leave a thread the registers it needs without spills (168
 // and 236 at head_dim 128).  At batch 64 with 3 CTAs: 554 us against 595 with
 // 4 and 128 spilling registers.
 template <int HD, int NT>
@@ -124,11 +122,11 @@ struct Join {
   unsigned *arrived;  // zero before and after a launch
 };
 
-template <int DT, int HD, int NT>
-__global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const __grid_constant__ PageAttnArgs a,
+template <int DT, int HD, int NT, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? kCtas<HD, NT> : 1) k_page_decode(const __grid_constant__ PageAttnArgs a,
                                                                             const __grid_constant__ Join j,
                                                                             const __grid_constant__ PrefixPartials x) {
-  constexpr int Q = 8 * NT;  // query columns
+  constexpr int Q = 8 * NT, kThreads = 32 * kWarps;  // query columns
   constexpr int CK = HD / 32, CV = HD / 64;
   __shared__ float so[kWarps][Q][HD];
   __shared__ float sm[kWarps][Q], sl[kWarps][Q];
@@ -140,6 +138,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   const int n_rank = j.ranks, c = blockIdx.x % n_rank, part = blockIdx.x / n_rank;  // rank in the cluster; cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
+  // behind the prefix's kernel, which has waited itself, the suffixes are read
+  // while that runs
+  if (!x.parts) mv::pdl_wait();
+  mv::pdl_launch_dependents();
   // the row, and the positions up to its own
   int r = b, rows = 1;
   bool bad = false;
@@ -483,22 +485,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, NT>) k_page_decode(const _
   store(acc, top, sum);
 }
 
-template <int DT, int HD, int NT>
+template <int DT, int HD, int NT, int W>
 cudaError_t launch(const PageAttnArgs &a, const DecodePlan &pl, const Join &j, const PrefixPartials &x, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.split, pl.units / (a.B * a.max_rows), a.B * a.max_rows);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = j.ranks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  // behind the prefix's kernel: the suffixes are read while it runs
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = x.parts ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k_page_decode<DT, HD, NT>, a, j, x);
+  return launch_serve(k_page_decode<DT, HD, NT, W>, dim3(pl.split, pl.units / (a.B * a.max_rows), a.B * a.max_rows), 32 * W, 0, j.ranks,
+                      s, a, j, x);
 }
 
 }  // namespace pd
@@ -522,12 +512,15 @@ DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix) {
   //    32768, 8 KV heads: 554 us with 4 (2048 CTAs), 574 with 8, 645 with 2
   int split = 1;
   while (split < 128) {
-    const long per_warp = groups / (2 * split * pd::kWarps), ctas = units * split;
+    const long per_warp = groups / (2 * split * 4), ctas = units * split;
     if (2 * ctas <= 4 * 148 && per_warp >= 2) split *= 2;
     else if (split < 8 && ctas < 12 * 148 && per_warp * 16 * a.kv.head_dim * 4 >= 128 << 10) split *= 2;
     else break;
   }
   pl.split = split;
+  // 8 warps a CTA where each has an SM to itself and a warp its group: one sequence with
+  // 1024 positions in sight TODO
+  pl.warps = pl.nt == 1 && units * split <= 148 && groups > 4l * split ? 8 : 4;
   if (split > 8) {
     const size_t n = (size_t)units * (split / 8);
     pl.o_bytes = n * q * a.kv.head_dim * sizeof(float);
@@ -551,12 +544,15 @@ int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, const DecodePlan &pl
   }
   const bool h = a.kv.dtype == TCB_F16, wide = a.kv.head_dim == 128;
   cudaError_t e;
-  if (pl.nt == 1) {
-    if (wide) e = h ? pd::launch<TCB_F16, 128, 1>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 1>(a, pl, j, x, s);
-    else e = h ? pd::launch<TCB_F16, 64, 1>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 1>(a, pl, j, x, s);
+  if (pl.warps == 8) {
+    if (wide) e = h ? pd::launch<TCB_F16, 128, 1, 8>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 1, 8>(a, pl, j, x, s);
+    else e = h ? pd::launch<TCB_F16, 64, 1, 8>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 1, 8>(a, pl, j, x, s);
+  } else if (pl.nt == 1) {
+    if (wide) e = h ? pd::launch<TCB_F16, 128, 1, 4>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 1, 4>(a, pl, j, x, s);
+    else e = h ? pd::launch<TCB_F16, 64, 1, 4>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 1, 4>(a, pl, j, x, s);
   } else {
-    if (wide) e = h ? pd::launch<TCB_F16, 128, 2>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 2>(a, pl, j, x, s);
-    else e = h ? pd::launch<TCB_F16, 64, 2>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 2>(a, pl, j, x, s);
+    if (wide) e = h ? pd::launch<TCB_F16, 128, 2, 4>(a, pl, j, x, s) : pd::launch<TCB_BF16, 128, 2, 4>(a, pl, j, x, s);
+    else e = h ? pd::launch<TCB_F16, 64, 2, 4>(a, pl, j, x, s) : pd::launch<TCB_BF16, 64, 2, 4>(a, pl, j, x, s);
   }
   return e == cudaSuccess ? TCB_OK : ctx_fail(ctx, e);
 }

@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   const int part = blockIdx.x % p.split, tile = p.tiles - 1 - (int)(blockIdx.x / p.split);  // the longest first
   const int kh = blockIdx.y, b = blockIdx.z;
 
+  mv::pdl_wait();
+  mv::pdl_launch_dependents();  // a kernel of suffixes waits again before it reads the partials
   // the request's rows
   int r0 = 0, n = a.T, len = 0;
   if (!p.joined) {
@@ -260,7 +262,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     n = min(n, a.max_rows);
   }
   const int x0 = tile * kTiles * kRows, rows = n * p.G;  // (row, head) pairs: fewer than the bytes of q
-  if (p.joined) mv::pdl_launch_dependents();  // the kernel of the suffixes, which waits before it reads the partials
   if (x0 >= rows) return;
   const int n_real = p.joined ? n : min(max(a.row_start[b + 1], r0), a.T) - r0;  // positions count from the true number of rows
   const int active = rows - x0 > kRows ? 2 : 1;  // query tiles with rows
@@ -689,6 +690,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
 // (4 elements a thread; H * HD / 4 threads a row)
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) k_rows_join(const PageAttnArgs a, int split, const float *po, const float2 *pml) {
+  mv::pdl_wait();
+  mv::pdl_launch_dependents();
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const long row = i / (HD / 4);
   if (row >= (long)a.T * a.H) return;
@@ -730,12 +733,12 @@ template <int DT, int HD>
 cudaError_t launch(const Args &p, dim3 grid, cudaStream_t s) {
   static const cudaError_t attr = cudaFuncSetAttribute(k_page_rows<DT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD>::kSmem);
   if (attr != cudaSuccess) return attr;
-  k_page_rows<DT, HD><<<grid, kThreads, Layout<HD>::kSmem, s>>>(p);
-  if (p.po && !p.joined) {
+  cudaError_t e = launch_serve(k_page_rows<DT, HD>, grid, kThreads, Layout<HD>::kSmem, 1, s, p);
+  if (e == cudaSuccess && p.po && !p.joined) {
     const long n = (long)p.a.T * p.a.H * (HD / 4);
-    k_rows_join<DT, HD><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p.a, p.split, p.po, p.pml);
+    e = launch_serve(k_rows_join<DT, HD>, dim3((unsigned)((n + 255) / 256)), 256, 0, 1, s, p.a, p.split, p.po, p.pml);
   }
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace pr

@@ -1,6 +1,8 @@
 // tcb_serve.cu - the serving operators' C entry points (page plan, K/V
 // append, attention over the pages) with their argument checks, and the
 // kernels of the plan and the append.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -10,6 +12,7 @@
 #include "../../include/tcb.h"
 #include "tcb_common.cuh"
 #include "tcb_ctx.h"
+#include "tcb_mv_ptx.cuh"
 #include "tcb_page.h"
 
 namespace {
@@ -75,26 +78,33 @@ __global__ void __launch_bounds__(NT) k_page_plan(const PlanArgs a) {
   extern __shared__ int sh[];
   int *rs = sh;              // [B + 1] first row of each request
   int *pg = sh + a.B + 1;    // [B] pages taken before it; -1: refused
+  int *cs = pg + a.B;        // [B] positions cached
   __shared__ long sums[NT / 32];
   __shared__ int taken_s;
   __shared__ long long asked_s;
+  tcb::mv::pdl_wait();
+  tcb::mv::pdl_launch_dependents();
   const int tid = threadIdx.x;
   const int items = (a.B + NT - 1) / NT;
   const int b0 = tid * items, b1 = min(a.B, b0 + items);
   const long n_free = min(max(*a.n_free, 0), a.free_cap);
   if (tid == 0) taken_s = 0, asked_s = 0;
 
+  // the lengths, read once where a thread has one request
+  const int c0 = b0 < b1 ? a.cached[b0] : 0, f0 = b0 < b1 ? a.fresh[b0] : 0;
+  auto cached = [&](int b) { return b == b0 ? c0 : a.cached[b]; };
+  auto fresh = [&](int b) { return b == b0 ? f0 : a.fresh[b]; };
   long sum = 0, total;
-  for (int b = b0; b < b1; b++) sum += max(a.fresh[b], 0);
+  for (int b = b0; b < b1; b++) sum += max(fresh(b), 0);
   long row = block_scan<NT>(sum, sums, total);
   // the pages each request lacks, 0 where it does not fit its rows or table
   const long r0 = row;
   long lacks = 0;
   for (int b = b0; b < b1; b++) {
-    const long f = a.fresh[b];
+    const long f = fresh(b);
     rs[b] = (int)min(row, (long)a.rows);
     row += max(f, 0l);
-    lacks += max(pages_lacking(a, a.cached[b], f, row), 0l);
+    lacks += max(pages_lacking(a, cached(b), f, row), 0l);
   }
   if (tid == 0) rs[a.B] = (int)min(total, (long)a.rows);
   long page = block_scan<NT>(lacks, sums, total);
@@ -102,7 +112,8 @@ __global__ void __launch_bounds__(NT) k_page_plan(const PlanArgs a) {
   int taken = 0;       // by the last request that gets pages
   long long asked = 0;  // up to the last one that is not refused
   for (int b = b0; b < b1; b++) {
-    const long c = a.cached[b], f = a.fresh[b];
+    const long c = cached(b), f = fresh(b);
+    cs[b] = (int)c;
     row += max(f, 0l);
     const long need = pages_lacking(a, c, f, row);
     const bool granted = need == 0 || (need > 0 && page + need <= n_free);
@@ -128,7 +139,7 @@ __global__ void __launch_bounds__(NT) k_page_plan(const PlanArgs a) {
   const int warps = gridDim.x * (NT / 32), lane = tid & 31;
   for (int b = blockIdx.x * (NT / 32) + (tid >> 5); b < a.B; b += warps) {
     if (pg[b] < 0) continue;
-    const int c = a.cached[b];
+    const int c = cs[b];
     const int have = (int)(((long)c + a.page - 1) >> a.page_shift);
     const int need = (int)(((long)c + a.fresh[b] + a.page - 1) >> a.page_shift) - have;
     for (int j = lane; j < need; j += 32) a.tables[b * a.ldt + have + j] = a.free_pages[n_free - 1 - pg[b] - j];
@@ -146,7 +157,7 @@ __global__ void __launch_bounds__(NT) k_page_plan(const PlanArgs a) {
         else hi = mid;
       }
       if (pg[lo] >= 0) {
-        const int c = a.cached[lo];
+        const int c = cs[lo];
         pos = c + (int)(r - rs[lo]);
         const int have = (int)(((long)c + a.page - 1) >> a.page_shift), at = pos >> a.page_shift;
         const int g = at < have ? a.tables[lo * a.ldt + at] : a.free_pages[n_free - 1 - pg[lo] - (at - have)];
@@ -188,6 +199,22 @@ __device__ __forceinline__ uint4 load_cache8(const void *x, long i, int dtype) {
   float f[8];
   load8<XT, VEC>(x, i, f);
   uint32_t o[4];
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 8; e++) nan |= f[e] != f[e];
+  if (!nan) {  // the conversions differ from the library's rounding in a NaN's payload alone
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (dtype == TCB_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+        o[e] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+        o[e] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
 #pragma unroll
   for (int e = 0; e < 4; e++)
     o[e] = dtype == TCB_BF16 ? tcb::f32_to_bf16(f[2 * e]) | (uint32_t)tcb::f32_to_bf16(f[2 * e + 1]) << 16
@@ -206,6 +233,8 @@ template <int XT, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const tcb_kv_pages kv, int page_shift, int T, const void *k,
                                                               long ldk, const void *v, long ldv, const int64_t *slots,
                                                               int *derr) {
+  tcb::mv::pdl_wait();
+  tcb::mv::pdl_launch_dependents();
   const int per_head = kv.head_dim / 8, places = kv.n_kv_heads * per_head;
   const int across = min(places, kAppendThreads);  // threads along a row; the CTA's other threads take other rows
   const int c = blockIdx.y * across + threadIdx.x % across, sub = threadIdx.x / across, rows = kAppendThreads / across;
@@ -292,18 +321,18 @@ int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached, const int *f
   if (rc != TCB_OK) return rc;
   PlanArgs a{B, page, log2i(page), width, free_cap, rows, cached, fresh, tables, ldt, free_pages, n_free,
              row_start, kv_len, slots, positions, balance, taken};
-  const size_t smem = (2 * (size_t)B + 1) * sizeof(int);
+  const size_t smem = (3 * (size_t)B + 1) * sizeof(int);
   // 128 threads while each has at most one request (4.1 us for 16 requests), else
   // 1024 (1024 requests with 110 thousand rows: 6.9 us, 8.2 with 256)
   auto go = [&](auto kernel, int nt, int most) {
     if (smem > 48 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (2 * TCB_PAGE_PLAN_MAX + 1) * (int)sizeof(int));
+                                                 (3 * TCB_PAGE_PLAN_MAX + 1) * (int)sizeof(int));
       if (e != cudaSuccess) return e;
     }
     const long want = std::max<long>((rows + nt - 1) / nt, (B + nt / 32 - 1) / (nt / 32));
-    kernel<<<(unsigned)std::min<long>(std::max<long>(want, 1), most), nt, smem, static_cast<cudaStream_t>(stream)>>>(a);
-    return cudaGetLastError();
+    return tcb::launch_serve(kernel, dim3((unsigned)std::min<long>(std::max<long>(want, 1), most)), nt, smem, 1,
+                             static_cast<cudaStream_t>(stream), a);
   };
   const cudaError_t e = B <= 128 ? go(k_page_plan<128>, 128, 8 * ctx->sms) : go(k_page_plan<1024>, 1024, ctx->sms);
   return e == cudaSuccess ? TCB_OK : tcb::ctx_fail(ctx, e);
@@ -329,11 +358,13 @@ int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k, lo
   const dim3 grid((unsigned)std::min<long>(waves, most), (unsigned)((places + across - 1) / across));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sh = log2i(kv->page);
-  auto go = [&](auto kernel) { kernel<<<grid, kAppendThreads, 0, s>>>(*kv, sh, T, k, ldk, v, ldv, slots, ctx->derr); };
-  if (xdtype == TCB_F32) vec ? go(k_kv_append<TCB_F32, true>) : go(k_kv_append<TCB_F32, false>);
-  else if (xdtype == TCB_F16) vec ? go(k_kv_append<TCB_F16, true>) : go(k_kv_append<TCB_F16, false>);
-  else vec ? go(k_kv_append<TCB_BF16, true>) : go(k_kv_append<TCB_BF16, false>);
-  cudaError_t e = cudaGetLastError();
+  auto go = [&](auto kernel) {
+    return tcb::launch_serve(kernel, grid, kAppendThreads, 0, 1, s, *kv, sh, T, k, ldk, v, ldv, slots, ctx->derr);
+  };
+  cudaError_t e;
+  if (xdtype == TCB_F32) e = vec ? go(k_kv_append<TCB_F32, true>) : go(k_kv_append<TCB_F32, false>);
+  else if (xdtype == TCB_F16) e = vec ? go(k_kv_append<TCB_F16, true>) : go(k_kv_append<TCB_F16, false>);
+  else e = vec ? go(k_kv_append<TCB_BF16, true>) : go(k_kv_append<TCB_BF16, false>);
   return e == cudaSuccess ? TCB_OK : tcb::ctx_fail(ctx, e);
 }
 
