@@ -518,9 +518,11 @@ DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix) {
     else break;
   }
   pl.split = split;
-  // 8 warps a CTA where each has an SM to itself and a warp its group: one sequence with
-  // 1024 positions in sight TODO
-  pl.warps = pl.nt == 1 && units * split <= 148 && groups > 4l * split ? 8 : 4;
+  // 8 warps a CTA where each CTA has an SM to itself and a warp its group: with 8 KV
+  // heads, one sequence of 1000 positions takes 7.8 us a call with 8 warps and
+  // 9.0 with 4, four of them 8.0 and 9.6.  Clusters of 8 such CTAs find room for
+  // fewer than 16 at once (128 CTAs: 17.4 us with 8 warps, 12.1 with 4).
+  pl.warps = pl.nt == 1 && groups > 4l * split && units * split <= (split >= 8 ? 64 : 148) ? 8 : 4;
   if (split > 8) {
     const size_t n = (size_t)units * (split / 8);
     pl.o_bytes = n * q * a.kv.head_dim * sizeof(float);
