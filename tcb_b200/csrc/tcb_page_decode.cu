@@ -504,16 +504,17 @@ DecodePlan page_decode_plan(const PageAttnArgs &a, bool suffix) {
   const long units = (long)a.B * a.max_rows * a.kv.n_kv_heads * ((G + q - 1) / q);
   pl.units = (int)units;
   // CTAs per unit, doubled
-  //  - while one wave of CTAs holds them (about 4 a SM) and a warp keeps 2 groups: one
+  //  - while one wave of CTAs holds them and a warp keeps 2 groups: one
   //    sequence with 1024 positions in sight takes 8.2 us with 8, 9.4 with 4;
   //    one of 32768 with one KV head 17.1 with 128, 64.9 with 8
   //  - up to a cluster, while there are fewer than about 4 waves and a warp keeps
   //    128 KB of K and V, to even out ragged lengths: 64 sequences of up to
   //    32768, 8 KV heads: 554 us with 4 (2048 CTAs), 574 with 8, 645 with 2
+  const long room = 148l * ((pl.nt == 1 ? 4 : 3) - (a.kv.head_dim == 128));
   int split = 1;
   while (split < 128) {
     const long per_warp = groups / (2 * split * 4), ctas = units * split;
-    if (2 * ctas <= 4 * 148 && per_warp >= 2) split *= 2;
+    if (2 * ctas <= room && per_warp >= 2) split *= 2;
     else if (split < 8 && ctas < 12 * 148 && per_warp * 16 * a.kv.head_dim * 4 >= 128 << 10) split *= 2;
     else break;
   }
