@@ -321,8 +321,10 @@ int tcb_llama_batch_logits(tcb_llama_batch *b, float **logits);
  * TCB_ERR_BOUNDS in the device error word (tcb_device_error) and touch
  * nothing outside the caller's arrays; the outputs of the request concerned
  * are then unspecified.  Scratch is the context's: order calls on one context
- * on one stream, and make one eager call of the largest shape before a
- * stream capture. */
+ * on one stream.  A call that needs more of it than any before allocates (not
+ * while a stream is captured: make one eager call of the shape first), and
+ * what is outgrown stays until the context goes, so captured graphs keep
+ * what they name. */
 
 /* A paged K/V cache: two pools of n_pages pages of `page` positions.  Element
  * d of KV head h at position t of page g is at

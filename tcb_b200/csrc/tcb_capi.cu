@@ -61,7 +61,7 @@ int ensure_ws(tcb_ctx *ctx, size_t bytes) {
   return TCB_OK;
 }
 
-// grow one of the context's staging buffers to `bytes`
+// grow one of the context's staging buffers (tcb_qgemm_host) to `bytes`
 int ensure_buf(tcb_ctx *ctx, void **buf, size_t *cap, size_t bytes) {
   if (bytes <= *cap) return TCB_OK;
   if (*buf) {
@@ -257,19 +257,34 @@ int qgemm_tc_prologue(tcb_ctx *ctx, int wtype, int M, int N, int K, const void *
 namespace tcb {
 int ctx_fail(tcb_ctx *ctx, cudaError_t e) { return cuda_fail(ctx, e); }
 int ctx_bind(tcb_ctx *ctx) { return bind(ctx); }
-int ctx_ws(tcb_ctx *ctx, size_t bytes) {
+// grow one of the kept buffers to at least `bytes`
+static int grow_kept(tcb_ctx *ctx, tcb_ctx::Kept &k, size_t bytes, bool zeroed) {
   std::lock_guard<std::mutex> lock(ctx->mu);
-  return ensure_ws(ctx, bytes);
-}
-int ctx_tick(tcb_ctx *ctx, size_t bytes) {
-  std::lock_guard<std::mutex> lock(ctx->mu);
-  if (bytes <= ctx->tick_cap) return TCB_OK;
-  int rc = ensure_buf(ctx, &ctx->tick, &ctx->tick_cap, bytes);
-  if (rc != TCB_OK) return rc;
-  TCB_CU(ctx, cudaMemset(ctx->tick, 0, ctx->tick_cap));
-  TCB_CU(ctx, cudaDeviceSynchronize());  // before a launch on any stream
+  if (bytes <= k.cap) return TCB_OK;
+  const size_t cap = std::max<size_t>(std::max<size_t>(bytes, 2 * k.cap), 64u << 10);
+  if (k.p && k.n_old == (int)(sizeof k.old / sizeof k.old[0])) return TCB_ERR_NOMEM;
+  void *p = nullptr;
+  cudaError_t e = cudaMalloc(&p, cap);
+  if (e != cudaSuccess) {
+    cuda_fail(ctx, e);
+    (void)cudaGetLastError();
+    return TCB_ERR_NOMEM;
+  }
+  if (zeroed) {  // before a launch on any stream
+    e = cudaMemset(p, 0, cap);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+      cudaFree(p);
+      return cuda_fail(ctx, e);
+    }
+  }
+  if (k.p) k.old[k.n_old++] = k.p;
+  k.p = p;
+  k.cap = cap;
   return TCB_OK;
 }
+int ctx_scratch(tcb_ctx *ctx, size_t bytes) { return grow_kept(ctx, ctx->sv, bytes, false); }
+int ctx_tick(tcb_ctx *ctx, size_t bytes) { return grow_kept(ctx, ctx->tick, bytes, true); }
 }  // namespace tcb
 
 namespace {
@@ -349,8 +364,11 @@ int tcb_ctx_destroy(tcb_ctx *ctx) {
   if (!ctx) return TCB_OK;
   int rc = TCB_OK;
   if (cudaSetDevice(ctx->dev) != cudaSuccess) rc = TCB_ERR_CUDA;
-  for (void *p : {ctx->ws, (void *)ctx->derr, ctx->sk, ctx->hx, ctx->hc, ctx->tick})
+  for (void *p : {ctx->ws, (void *)ctx->derr, ctx->sk, ctx->hx, ctx->hc, ctx->sv.p, ctx->tick.p})
     if (p && cudaFree(p) != cudaSuccess) rc = TCB_ERR_CUDA;
+  for (tcb_ctx::Kept *k : {&ctx->sv, &ctx->tick})
+    for (int i = 0; i < k->n_old; i++)
+      if (cudaFree(k->old[i]) != cudaSuccess) rc = TCB_ERR_CUDA;
   delete ctx;
   return rc;
 }

@@ -18,8 +18,16 @@ struct tcb_ctx {
   size_t hx_cap = 0;
   void *hc = nullptr;   // tcb_qgemm_host: c of a caller whose c the GPU cannot reach
   size_t hc_cap = 0;
-  void *tick = nullptr;  // arrival counters and pick words of the logits kernel (zeroed; launches leave it zeroed)
-  size_t tick_cap = 0;
+  // the serving operators' scratch, and their arrival counters and pick words
+  // (zeroed; launches leave them zeroed).  An outgrown buffer is kept until the
+  // context goes: a captured graph may still name it (each is at least twice the
+  // one before).
+  struct Kept {
+    void *p = nullptr;
+    size_t cap = 0;
+    void *old[64] = {nullptr};
+    int n_old = 0;
+  } sv, tick;
   std::mutex mu;
   char err[256] = {0};
 };
@@ -28,6 +36,6 @@ struct tcb_ctx {
 namespace tcb {
 int ctx_fail(tcb_ctx *ctx, cudaError_t e);        // record the error, TCB_ERR_CUDA
 int ctx_bind(tcb_ctx *ctx);                       // make the context's device current
-int ctx_ws(tcb_ctx *ctx, size_t bytes);           // at least `bytes` of scratch in ctx->ws
-int ctx_tick(tcb_ctx *ctx, size_t bytes);         // at least `bytes` of zeroed counters in ctx->tick
+int ctx_scratch(tcb_ctx *ctx, size_t bytes);      // at least `bytes` of scratch in ctx->sv.p
+int ctx_tick(tcb_ctx *ctx, size_t bytes);         // at least `bytes` of zeroed counters in ctx->tick.p
 }  // namespace tcb

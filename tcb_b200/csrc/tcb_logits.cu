@@ -276,7 +276,7 @@ extern "C" int tcb_logits_penalize(tcb_ctx *ctx, const tcb_logits_args *p, void 
   // per tile)
   int threads = 128;
   while (threads < kMaxThreads && (long)a.B * ((a.V + 2 * threads * kPer - 1) / (2 * threads * kPer)) >= 148) threads *= 2;
-  Pick *picks = static_cast<Pick *>(ctx->tick);
+  Pick *picks = static_cast<Pick *>(ctx->tick.p);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = a.dtype == TCB_F32   ? launch_to<TCB_F32>(a, threads, picks, ctx->derr, s)
                         : a.dtype == TCB_F16 ? launch_to<TCB_F16>(a, threads, picks, ctx->derr, s)

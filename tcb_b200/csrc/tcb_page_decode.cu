@@ -543,7 +543,7 @@ int launch_page_decode(tcb_ctx *ctx, const PageAttnArgs &a, const DecodePlan &pl
     if (rc != TCB_OK) return rc;
     j.o = static_cast<float *>(scratch);
     j.ml = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + pl.o_bytes);
-    j.arrived = static_cast<unsigned *>(ctx->tick);
+    j.arrived = static_cast<unsigned *>(ctx->tick.p);
   }
   const bool h = a.kv.dtype == TCB_F16, wide = a.kv.head_dim == 128;
   cudaError_t e;

@@ -391,12 +391,12 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H, con
   const double read = (double)B * a.max_rows * seen * kv->n_kv_heads * kv->head_dim * 4;
   if (a.max_rows == 1 || (read <= 20e6 && (long)B * a.max_rows <= 65535)) {
     const tcb::DecodePlan pl = tcb::page_decode_plan(a, false);
-    if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
-    return tcb::launch_page_decode(ctx, a, pl, ctx->ws, {}, s);
+    if ((rc = tcb::ctx_scratch(ctx, pl.bytes)) != TCB_OK) return rc;
+    return tcb::launch_page_decode(ctx, a, pl, ctx->sv.p, {}, s);
   }
   const tcb::RowsPlan pl = tcb::page_rows_plan(a);
-  if ((rc = tcb::ctx_ws(ctx, pl.bytes)) != TCB_OK) return rc;
-  return tcb::launch_page_rows(ctx, a, pl, ctx->ws, s);
+  if ((rc = tcb::ctx_scratch(ctx, pl.bytes)) != TCB_OK) return rc;
+  return tcb::launch_page_rows(ctx, a, pl, ctx->sv.p, s);
 }
 
 int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const void *q, long ldq, void *out, long ldo,
@@ -425,8 +425,8 @@ int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H, const vo
   tcb::RowsPlan rp{};
   if (apart) rp = tcb::page_rows_plan(a);
   const size_t at = (rp.bytes + 255) / 256 * 256;
-  if ((rc = tcb::ctx_ws(ctx, at + dp.bytes)) != TCB_OK) return rc;
-  char *ws = static_cast<char *>(ctx->ws);
+  if ((rc = tcb::ctx_scratch(ctx, at + dp.bytes)) != TCB_OK) return rc;
+  char *ws = static_cast<char *>(ctx->sv.p);
   tcb::PrefixPartials x{};
   if (apart) {
     if ((rc = tcb::launch_page_rows(ctx, a, rp, ws, s)) != TCB_OK) return rc;

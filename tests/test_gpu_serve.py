@@ -447,6 +447,27 @@ def test_attend_on_a_side_stream_and_in_a_graph(ctx):
     assert torch.equal(out, want)
 
 
+def test_captured_graphs_outlive_larger_calls():
+    """A graph names the scratch of its capture; a later call that needs more
+    leaves it in place."""
+    own = T.Context(0)
+    c = attn_case([3000], [1], 4, 1, 128, 64, F16, seed=5)
+    p = serve.Pages(own, c["k"], c["v"])
+    args = (c["row_start"], c["kv_len"], c["tables"], 1, 3000)
+    want, out = torch.empty_like(c["q"]), torch.zeros_like(c["q"])
+    p.attend(c["q"], want, *args)  # several clusters: joined through scratch and counters
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.attend(c["q"], out, *args)
+    d = attn_case([400] * 6, [200] * 6, 4, 1, 128, 64, F16, seed=6)
+    big = torch.empty_like(d["q"])
+    serve.Pages(own, d["k"], d["v"]).attend(d["q"], big, d["row_start"], d["kv_len"], d["tables"], 200, 1 << 20)
+    run_logits(own, logits_case(3000, 40, 0, seed=1))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and own.device_error() == 0
+
+
 # ------------------------------------------------------------ shared prefix
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
