@@ -266,6 +266,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   const int n_real = p.joined ? n : min(max(a.row_start[b + 1], r0), a.T) - r0;  // positions count from the true number of rows
   const int active = rows - x0 > kRows ? 2 : 1;  // query tiles with rows
 
+  // softmax threads: the row and its Q, asked for before the setup (rows that do
+  // not exist are zero): a warp takes its 32 rows one after the other, HD / 8
+  // lanes a row
+  const int qt = (warp >> 2) - 1, tid = threadIdx.x & 127;  // warps 4-7: 0, 8-11: 1
+  const int x = x0 + qt * kRows + tid;
+  const bool live = qt >= 0 && x < rows;
+  const int xi = live ? (int)((unsigned)x / (unsigned)p.G) : 0;
+  const int head = kh * p.G + (live ? x - xi * p.G : 0);
+  const long r = r0 + xi;
+  constexpr int kLanes = HD / 8;
+  uint4 qv[kLanes];
+  if (qt >= 0) {
+    const long at = live && a.scale_log2 != 0.f ? r * a.ldq + (long)head * HD : -1;
+#pragma unroll
+    for (int i = 0; i < kLanes; i++) {
+      const long off = __shfl_sync(kAll, at, i * (32 / kLanes) + lane / kLanes);
+      qv[i] = make_uint4(0, 0, 0, 0);
+      if (off >= 0) qv[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + off + 8 * (lane % kLanes));
+    }
+  }
+
   if (threadIdx.x == 0) {
     hi_min = lo_min = first_min = 0x7FFFFFFF;
     hi_max = lo_max = first_max = 0;
@@ -295,13 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   }
   __syncthreads();
 
-  // softmax threads: the row, what it sees, and its Q
-  const int qt = (warp >> 2) - 1, tid = threadIdx.x & 127;  // warps 4-7: 0, 8-11: 1
-  const int x = x0 + qt * kRows + tid;
-  const bool live = qt >= 0 && x < rows;
-  const int xi = live ? (int)((unsigned)x / (unsigned)p.G) : 0;
-  const int head = kh * p.G + (live ? x - xi * p.G : 0);
-  const long r = r0 + xi;
+  // what the row sees
   int hi = 0, lo = 0, first = 0;
   if (live) {
     if (p.joined) {
@@ -496,25 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // Q into the swizzled tile (rows that do not exist are zero): the warp takes
-    // its 32 rows one after the other, HD / 8 lanes a row
+    // Q into the swizzled tile
     if (qt < active) {
-      const long at = live && a.scale_log2 != 0.f ? r * a.ldq + (long)head * HD : -1;
       const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-      constexpr int kLanes = HD / 8;
-      const int c = lane % kLanes;
-      uint4 v[kLanes];
 #pragma unroll
       for (int i = 0; i < kLanes; i++) {
-        const long off = __shfl_sync(kAll, at, i * (32 / kLanes) + lane / kLanes);
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (off >= 0) v[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + off + 8 * c);
-      }
-#pragma unroll
-      for (int i = 0; i < kLanes; i++) {
-        const int row = (warp & 3) * 32 + i * (32 / kLanes) + lane / kLanes;
-        v[i].x ^= sign, v[i].y ^= sign, v[i].z ^= sign, v[i].w ^= sign;
-        *reinterpret_cast<uint4 *>(sm + L::kQ + qt * L::kTile + row * 128 + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)) = v[i];
+        const int row = (warp & 3) * 32 + i * (32 / kLanes) + lane / kLanes, c = lane % kLanes;
+        qv[i].x ^= sign, qv[i].y ^= sign, qv[i].z ^= sign, qv[i].w ^= sign;
+        *reinterpret_cast<uint4 *>(sm + L::kQ + qt * L::kTile + row * 128 + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)) = qv[i];
       }
       mv::fence_proxy_async();
     }
@@ -612,12 +616,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       const float inv = p.po ? 1.f : __fdiv_rn(1.f, empty ? 1.f : l);
       const long prow = ((long)part * a.T + r) * a.H + head;
       if (p.po && live) p.pml[prow] = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
+      uint32_t ahead[32];  // the next 32 columns, on their way while these are written
+      if (iters > 0 && ok) tmem_ld(to_addr, ahead);
 #pragma unroll 1
       for (int c = 0; c < HD / 32 && ok; c++) {
         uint32_t o[32];
         if (iters > 0) {
-          tmem_ld(to_addr + 32 * c, o);
-          tmem_wait_ld(o);
+          tmem_wait_ld(ahead);
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = ahead[j];
+          if (c + 1 < HD / 32) tmem_ld(to_addr + 32 * (c + 1), ahead);
         }
 #pragma unroll
         for (int j = 0; j < 32; j++) o[j] = empty ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
