@@ -322,8 +322,8 @@ int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached, const int *f
   PlanArgs a{B, page, log2i(page), width, free_cap, rows, cached, fresh, tables, ldt, free_pages, n_free,
              row_start, kv_len, slots, positions, balance, taken};
   const size_t smem = (3 * (size_t)B + 1) * sizeof(int);
-  // 128 threads while each has at most one request (4.1 us for 16 requests), else
-  // 1024 (1024 requests with 110 thousand rows: 6.9 us, 8.2 with 256)
+  // 128 threads while each has at most one request (3.4 us for 16 requests), else
+  // 1024 (1024 requests with 110 thousand rows: 6.8 us, 8.2 with 256)
   auto go = [&](auto kernel, int nt, int most) {
     if (smem > 48 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
