@@ -388,8 +388,9 @@ int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k,
  * a row does not look, NaN included, does not reach its result.
  *   q, out     T rows of H heads of head_dim elements in the cache's type, ldq
  *              and ldo elements apart; 16-byte aligned rows
- *   row_start  device [B + 1], as tcb_page_plan writes it; rows of q outside
- *              every request are left alone
+ *   row_start  device [B + 1], as tcb_page_plan writes it (starts that fall are
+ *              reported, TCB_ERR_BOUNDS); rows of q outside every request are
+ *              left alone
  *   kv_len     device [B], positions in the cache with this step's rows
  *   tables     device [B][width] page numbers, rows ldt apart
  *   max_rows   no request has more rows (1: a decode step)

@@ -63,6 +63,8 @@ struct PageAttnArgs {
 // pairs [split][T * H]; a prefix's are joined by the kernel of its suffixes.
 struct RowsPlan {
   int tiles, split;
+  long items;   // pairs of query tiles that have CTAs (for each KV head and part)
+  bool packed;  // counted over all requests
   bool partial;
   size_t o_bytes, bytes;
 };

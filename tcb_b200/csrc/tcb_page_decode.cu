@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? kCtas<HD, NT> : 1) 
     const int r0 = min(max(a.row_start[b], 0), a.T);
     rows = min(max(a.row_start[b + 1], r0), a.T) - r0;
     r = r0 + at;
-    bad = rows > a.max_rows;
+    bad = rows > a.max_rows || a.row_start[b + 1] < a.row_start[b];
   }
   const bool live = at < rows;
   int len = a.kv_len[b];

@@ -41,6 +41,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tcb_common.cuh"
 #include "tcb_mv_ptx.cuh"
@@ -237,7 +238,49 @@ struct Layout {
   static constexpr int kSmem = kBars + (int)sizeof(Bars) + 64 + 1024;
 };
 
-template <int DT, int HD>
+// Pair of query tiles number `item` of all requests in order, by the whole warp:
+// its request, and which of that request's it is (the last, the longest, first).
+// False: there are only `upto` of them.
+constexpr int kEach = 4;  // requests a lane looks at at once
+__device__ __forceinline__ bool find(const Args &p, int item, int &b, int &tile, long &upto) {
+  const PageAttnArgs &a = p.a;
+  const int lane = threadIdx.x & 31;
+  upto = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32 * kEach) {
+    const int mine = b0 + kEach * lane;
+    int rs[kEach + 1], n[kEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e <= kEach; e++) rs[e] = a.row_start[min(mine + e, a.B)];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      const int r0 = min(max(rs[e], 0), a.T), rows = min(min(max(rs[e + 1], r0), a.T) - r0, a.max_rows) * p.G;
+      n[e] = mine + e < a.B ? (rows + kTiles * kRows - 1) / (kTiles * kRows) : 0;
+      sum += n[e];
+    }
+    int to = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int v = __shfl_up_sync(kAll, to, d);
+      if (lane >= d) to += v;
+    }
+    const uint32_t at = __ballot_sync(kAll, item < upto + to);
+    if (at) {
+      int off = (int)(item - (upto + to - sum)), e = 0;
+#pragma unroll
+      for (int i = 0; i < kEach - 1; i++)
+        if (e == i && off >= n[i]) off -= n[i], e++;
+      const int left = e == 0 ? n[0] : e == 1 ? n[1] : e == 2 ? n[2] : n[3];
+      b = __shfl_sync(kAll, mine + e, __ffs(at) - 1);
+      tile = __shfl_sync(kAll, left - 1 - off, __ffs(at) - 1);
+      return true;
+    }
+    upto += __shfl_sync(kAll, to, 31);
+  }
+  return false;
+}
+
+// kPacked: CTAs count the requests' pairs of tiles (find), not tiles for each request
+template <int DT, int HD, bool kPacked>
 __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant__ Args p) {
   using L = Layout<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -247,14 +290,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   __shared__ int hi_min, hi_max, lo_min, lo_max, first_min, first_max;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int stop;
-  __shared__ int dirty;
+  __shared__ int dirty, request;
   const PageAttnArgs &a = p.a;
   const int warp = __shfl_sync(kAll, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the warp's number in a uniform register
-  const int part = blockIdx.x % p.split, tile = p.tiles - 1 - (int)(blockIdx.x / p.split);  // the longest first
-  const int kh = blockIdx.y, b = blockIdx.z;
+  const int part = blockIdx.x % p.split, kh = blockIdx.y;
+  int tile = p.tiles - 1 - (int)(blockIdx.x / p.split), b = blockIdx.z;  // the longest first
 
   mv::pdl_wait();
   mv::pdl_launch_dependents();  // a kernel of suffixes waits again before it reads the partials
+  if constexpr (kPacked) {
+    long upto;
+    if (blockIdx.x + blockIdx.y == 0 && warp == 0) {
+      // requests without rows have no CTA that looks at their lengths; row
+      // starts that fall may hold more tiles than there are CTAs
+      for (int i = lane; i < a.B; i += 32) {
+        const int l = a.kv_len[i];
+        if (l < 0 || l > a.max_len || l > (long)a.width << a.page_shift || a.row_start[i + 1] < a.row_start[i]) atomicExch(a.derr, TCB_ERR_BOUNDS);
+      }
+    }
+    if (!find(p, (int)(blockIdx.x / p.split), b, tile, upto)) return;
+  }
   // the request's rows
   int r0 = 0, n = a.T, len = 0;
   if (!p.joined) {
@@ -262,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     n = min(max(a.row_start[b + 1], r0), a.T) - r0;
     len = a.kv_len[b];
     const bool bad = len < 0 || len > a.max_len || len > (long)a.width << a.page_shift;
-    if ((bad || n > a.max_rows) && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
+    if ((bad || n > a.max_rows || a.row_start[b + 1] < a.row_start[b]) && threadIdx.x == 0) atomicExch(a.derr, TCB_ERR_BOUNDS);
     if (bad) len = 0;
     n = min(n, a.max_rows);
   }
@@ -297,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
     hi_max = lo_max = first_max = 0;
     stop = 0;
     dirty = 0;
+    request = b;
     for (int i = 0; i < kStages; i++) {
       mbar_init(bar.kfull + i, 1);
       mbar_init(bar.kempty + i, 1);
@@ -636,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
         for (int j = 0; j < 32; j++) o[j] = empty ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
         if (dirty && live) {
           // the non-finite V elements of edge tiles, for the rows that see them
-          const int *table = p.joined ? a.prefix : a.tables + b * a.ldt;
+          const int *table = p.joined ? a.prefix : a.tables + request * a.ldt;
           for (int u = u0; u < u1; u++) {
             const int k0 = key_of(u);
             if (in_full_sight(k0)) continue;
@@ -743,10 +799,13 @@ bool tensor_map(CUtensorMap *tm, const tcb_kv_pages &kv, const void *base, int b
 }
 
 template <int DT, int HD>
-cudaError_t launch(const Args &p, dim3 grid, cudaStream_t s) {
-  static const cudaError_t attr = cudaFuncSetAttribute(k_page_rows<DT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD>::kSmem);
-  if (attr != cudaSuccess) return attr;
-  cudaError_t e = launch_serve(k_page_rows<DT, HD>, grid, kThreads, Layout<HD>::kSmem, 1, s, p);
+cudaError_t launch(const Args &p, bool packed, dim3 grid, cudaStream_t s) {
+  auto go = [&](auto by_count) {
+    constexpr auto kernel = k_page_rows<DT, HD, decltype(by_count)::value>;
+    static const cudaError_t attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD>::kSmem);
+    return attr != cudaSuccess ? attr : launch_serve(kernel, grid, kThreads, Layout<HD>::kSmem, 1, s, p);
+  };
+  cudaError_t e = packed ? go(std::integral_constant<bool, true>()) : go(std::integral_constant<bool, false>());
   if (e == cudaSuccess && p.po && !p.joined) {
     const long n = (long)p.a.T * p.a.H * (HD / 4);
     e = launch_serve(k_rows_join<DT, HD>, dim3((unsigned)((n + 255) / 256)), 256, 0, 1, s, p.a, p.split, p.po, p.pml);
@@ -762,7 +821,17 @@ RowsPlan page_rows_plan(const PageAttnArgs &a) {
   const long rows = (long)(joined ? a.T : a.max_rows) * (a.H / a.kv.n_kv_heads);
   pl.tiles = (int)((rows + pr::kTiles * pr::kRows - 1) / (pr::kTiles * pr::kRows));
   const long seen = joined ? a.prefix_len : a.window < 0 ? a.max_len : std::min<long>(a.max_len, (long)a.window + a.sinks + 32);
-  const long keys = (seen + pr::kKeys - 1) / pr::kKeys, units = (long)pl.tiles * a.kv.n_kv_heads * (joined ? 1 : a.B);
+  // CTAs: the longest request's pairs of tiles for every request, many of which
+  // may be empty, or as many as the rows of all requests can fill, each of which
+  // then looks for its own (up to 1 us), where that spares 3 empty CTAs an SM.
+  // 256 requests of one row and one of 2048 (65000 spared): 920 us / 545; 4 of 64
+  // and one of 2048 (952): 85.7 / 80.0; 7 of 64 to 515 (336): 28.3 / 27.3, and in
+  // another case 29.7 / 30.9.
+  pl.items = pl.tiles * (joined ? 1l : a.B);
+  const long filled = (long)a.T * (a.H / a.kv.n_kv_heads) / (pr::kTiles * pr::kRows) + std::min(a.T, a.B);
+  pl.packed = !joined && (pl.items - filled) * a.kv.n_kv_heads >= 3 * 148;
+  if (pl.packed) pl.items = filled;
+  const long keys = (seen + pr::kKeys - 1) / pr::kKeys, units = std::max(1l, pl.items * a.kv.n_kv_heads);
   // CTAs along the positions where the others leave SMs idle, two tiles each at the least
   pl.split = (int)std::max<long>(1, std::min<long>(148 / units, keys / 2));
   if (joined) pl.split = std::min(pl.split, kMaxPrefixParts);
@@ -789,11 +858,11 @@ int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, vo
   }
   if (!pr::tensor_map(&p.tk, a.kv, a.kv.k, p.box) || !pr::tensor_map(&p.tv, a.kv, a.kv.v, p.box))
     return ctx_fail(ctx, cudaErrorInvalidValue);
-  const dim3 grid(p.tiles * p.split, a.kv.n_kv_heads, p.joined ? 1 : a.B);
+  const dim3 grid((pl.packed ? (unsigned)pl.items : (unsigned)p.tiles) * p.split, a.kv.n_kv_heads, p.joined || pl.packed ? 1 : a.B);
   const bool h = a.kv.dtype == TCB_F16;
   cudaError_t e;
-  if (a.kv.head_dim == 128) e = h ? pr::launch<TCB_F16, 128>(p, grid, s) : pr::launch<TCB_BF16, 128>(p, grid, s);
-  else e = h ? pr::launch<TCB_F16, 64>(p, grid, s) : pr::launch<TCB_BF16, 64>(p, grid, s);
+  if (a.kv.head_dim == 128) e = h ? pr::launch<TCB_F16, 128>(p, pl.packed, grid, s) : pr::launch<TCB_BF16, 128>(p, pl.packed, grid, s);
+  else e = h ? pr::launch<TCB_F16, 64>(p, pl.packed, grid, s) : pr::launch<TCB_BF16, 64>(p, pl.packed, grid, s);
   return e == cudaSuccess ? TCB_OK : ctx_fail(ctx, e);
 }
 

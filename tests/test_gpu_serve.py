@@ -262,6 +262,68 @@ def test_attend_by_tiles(ctx, dtype, window, sinks, H, KVH, hd, page, layout):
     check_rows(out, c, lens, rows, dtype, window, sinks, 1 / math.sqrt(hd), "tiles")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (37, 0), (4, 64), (0, 0)])
+@pytest.mark.parametrize("H,KVH,hd,page", [(8, 2, 128, 16), (5, 1, 64, 64), (2, 2, 64, 32)])
+def test_attend_few_long_among_many(ctx, dtype, window, sinks, H, KVH, hd, page):
+    """Single rows, requests without rows and a few prompts: far fewer tiles
+    than the longest request's for every request."""
+    B = 300
+    rows = [(1, 1, 0, 2)[b % 4] for b in range(B)]
+    for b, m in ((5, 260), (127, 130), (128, 300), (129, 1), (299, 515)):
+        rows[b] = m
+    lens = [max(m, 3 + 7 * b % 90) for b, m in enumerate(rows)]
+    c = attn_case(lens, rows, H, KVH, hd, page, dtype, seed=H + hd + 3)
+    out = torch.full_like(c["q"], math.nan)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], 600, 70000, window=window, sinks=sinks)
+    check_rows(out, c, lens, rows, dtype, window, sinks, 1 / math.sqrt(hd), "among many")
+    assert ctx.device_error(clear=True) == 0
+
+
+@pytest.mark.parametrize("H,KVH,hd", [(1, 1, 64), (4, 1, 128)])
+def test_attend_few_requests_with_rows(ctx, H, KVH, hd):
+    """Most requests without rows, the positions of the others in parts."""
+    rows, lens = [0] * 40, [50] * 40
+    rows[3], rows[39], lens[3], lens[39] = 300, 5, 700, 1000
+    c = attn_case(lens, rows, H, KVH, hd, 16, BF16, seed=hd)
+    out = torch.full_like(c["q"], math.nan)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], 1000, 70000)
+    check_rows(out, c, lens, rows, BF16, None, 0, 1 / math.sqrt(hd), "few with rows")
+    # lengths of requests without rows are looked at too, and row starts that fall
+    p, bad = serve.Pages(ctx, c["k"], c["v"]), c["kv_len"].clone()
+    bad[7] = -1
+    p.attend(c["q"], out, c["row_start"], bad, c["tables"], 1000, 70000)
+    assert ctx.device_error(clear=True) == BOUNDS
+    check_rows(out, c, lens, rows, BF16, None, 0, 1 / math.sqrt(hd), "few with rows")
+    falls = c["row_start"].clone()
+    falls[20] = 0
+    p.attend(c["q"], out, falls, c["kv_len"], c["tables"], 1000, 70000)
+    assert ctx.device_error(clear=True) == BOUNDS
+
+
+@pytest.mark.parametrize("H,KVH,hd", [(1, 1, 64), (2, 1, 128), (4, 1, 64), (8, 2, 64)])
+def test_attend_one_prompt_among_requests_without_rows(ctx, H, KVH, hd):
+    """Few tiles, found by count, and the positions in parts."""
+    rows, lens = [0] * 40, [50] * 40
+    rows[3], rows[39], lens[3], lens[39] = 1990, 5, 2100, 1000
+    c = attn_case(lens, rows, H, KVH, hd, 16, F16, seed=hd + 1)
+    p, out = serve.Pages(ctx, c["k"], c["v"]), torch.full_like(c["q"], math.nan)
+    p.attend(c["q"], out, c["row_start"], c["kv_len"], c["tables"], 1995, 70000)
+    check_rows(out, c, lens, rows, F16, None, 0, 1 / math.sqrt(hd), "one prompt")
+    bad, falls = c["kv_len"].clone(), c["row_start"].clone()
+    bad[7], falls[20] = -1, 0
+    for start, n in ((c["row_start"], bad), (falls, c["kv_len"])):
+        assert ctx.device_error(clear=True) == 0
+        p.attend(c["q"], out, start, n, c["tables"], 1995, 70000)
+        assert ctx.device_error(clear=True) == BOUNDS
+
+
+def test_attend_row_starts_that_fall_single_rows(ctx):
+    c = attn_case([9, 9, 9], [1, 1, 1], 4, 2, 64, 16, F16)
+    serve.Pages(ctx, c["k"], c["v"]).attend(c["q"], torch.empty_like(c["q"]), i32([0, 2, 1, 2]), c["kv_len"], c["tables"], 2, 9)
+    assert ctx.device_error(clear=True) == BOUNDS
+
+
 @pytest.mark.parametrize("rows,n", [([1], 5000), ([1], 4097), ([2], 3000), ([200], 2100), ([517], 517), ([1030], 1500)])
 @pytest.mark.parametrize("dtype,H,KVH,hd", [(F16, 4, 1, 128), (BF16, 6, 2, 64)])
 def test_attend_longer(ctx, rows, n, dtype, H, KVH, hd):
