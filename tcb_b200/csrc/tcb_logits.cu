@@ -227,12 +227,12 @@ cudaError_t launch(const tcb_logits_args &a, int threads, Pick *picks, int *derr
   const dim3 grid((a.V + tile - 1) / tile, a.B);
   const size_t smem = (a.n_bias ? 2 : a.history ? 1 : 0) * tile * sizeof(uint32_t);
   auto go = [&](auto kernel) {
-    static const cudaError_t attr = [&] {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxThreads * kPer * 4);
-      return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    }();
-    if (attr != cudaSuccess) return attr;
-    return launch_serve(kernel, grid, threads, smem, 1, s, a, picks, derr);
+    // the attributes belong to the kernel on the current device: asked for with
+    // every launch that needs them
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxThreads * kPer * 4);
+    if (e == cudaSuccess && smem) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    return e != cudaSuccess ? e : launch_serve(kernel, grid, threads, smem, 1, s, a, picks, derr);
   };
   return vec ? go(k_penalize<XT, OT, true>) : go(k_penalize<XT, OT, false>);
 }
