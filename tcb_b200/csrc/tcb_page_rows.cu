@@ -802,8 +802,9 @@ template <int DT, int HD>
 cudaError_t launch(const Args &p, bool packed, dim3 grid, cudaStream_t s) {
   auto go = [&](auto by_count) {
     constexpr auto kernel = k_page_rows<DT, HD, decltype(by_count)::value>;
-    static const cudaError_t attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD>::kSmem);
-    return attr != cudaSuccess ? attr : launch_serve(kernel, grid, kThreads, Layout<HD>::kSmem, 1, s, p);
+    // the attribute belongs to the kernel on the current device
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD>::kSmem);
+    return e != cudaSuccess ? e : launch_serve(kernel, grid, kThreads, Layout<HD>::kSmem, 1, s, p);
   };
   cudaError_t e = packed ? go(std::integral_constant<bool, true>()) : go(std::integral_constant<bool, false>());
   if (e == cudaSuccess && p.po && !p.joined) {
