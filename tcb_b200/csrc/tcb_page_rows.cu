@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
   int tile = p.tiles - 1 - (int)(blockIdx.x / p.split), b = blockIdx.z;  // the longest first
 
   mv::pdl_wait();
-  mv::pdl_launch_dependents();  // a kernel of suffixes waits again before it reads the partials
+  mv::pdl_launch_dependents();
   if constexpr (kPacked) {
     long upto;
     if (blockIdx.x + blockIdx.y == 0 && warp == 0) {
