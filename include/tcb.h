@@ -392,7 +392,8 @@ int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k,
  *              reported, TCB_ERR_BOUNDS); rows of q outside every request are
  *              left alone
  *   kv_len     device [B], positions in the cache with this step's rows
- *   tables     device [B][width] page numbers, rows ldt apart
+ *   tables     device [B][width] page numbers, rows ldt apart; entries of pages that no
+ *              row of the request sees (behind the window) may hold anything
  *   max_rows   no request has more rows (1: a decode step)
  *   max_len    no kv_len is larger
  * Scores, softmax statistics and sums are in f32; the weights p_j are rounded

@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       hi = max(pos + 1, 0);
       lo = a.window < 0 ? 0 : (int)min((long)hi, max(0l, (long)pos - a.window + 1));
       first = min(a.sinks, lo);
-      if (first == lo) lo = first = 0;
+      if (lo == hi) hi = first, lo = 0;  // no window: the first positions alone
+      if (first >= lo) lo = first = 0;
     }
   }
   if (qt >= 0) {
@@ -427,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       const int *table = p.joined ? a.prefix : a.tables + b * a.ldt;
       auto page_at = [&](int u) {
         const int pos = key_of(u) + at * p.box;
-        if (u >= u1 || !mine || pos >= hi_max) return a.kv.n_pages;  // outside the pools: zeros
+        // outside the pools: zeros, for what no row sees (its pages may have been given back)
+        if (u >= u1 || !mine || pos >= hi_max || (pos >= first_max && pos + p.box <= lo_min)) return a.kv.n_pages;
         const int pg = table[pos >> a.page_shift];
         if (pg >= 0 && pg < a.kv.n_pages) return pg;
         atomicExch(a.derr, TCB_ERR_BOUNDS);
