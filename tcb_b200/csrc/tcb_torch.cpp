@@ -214,7 +214,9 @@ int attend_prefix(PyObject *const *a) {
   if (!q.typed) return TCB_ERR_DTYPE;
   const int prefix_len = whole32(a[6], "prefix_len");
   need(prefix_len >= 0, "prefix_len: a whole number from 0 is wanted");
-  const int *prefix = vec<int>(a[5], ((int64_t)prefix_len + kv->page - 1) / kv->page, at::kInt, dev, "prefix");
+  // pools without positions are the entry's to refuse
+  const int64_t pages = kv->page > 0 ? ((int64_t)prefix_len + kv->page - 1) / kv->page : 0;
+  const int *prefix = vec<int>(a[5], pages, at::kInt, dev, "prefix");
   const int *kv_len = vec<int>(a[7], q.T, at::kInt, dev, "kv_len");
   const Rows t = rows(a[8], at::kInt, dev, "tables");
   need(t.n >= q.T, "tables: a row per request is wanted");
