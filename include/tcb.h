@@ -359,8 +359,9 @@ typedef struct tcb_kv_pages {
  * or the `rows` entries of slots do not hold it, or the free pages end before
  * it has its share (as later ones that lack pages are then); it takes no
  * page.  need is 0 for one that is refused on its lengths, rows or table.  The
- * inputs are not changed (balance and taken are not the array n_free): the
- * same call again gives the same. */
+ * inputs are not changed, so the same call again gives the same; outputs that
+ * overlap an input, the tables or one another are refused (kv_len is not the
+ * array cached: copy it there afterwards). */
 #define TCB_PAGE_PLAN_MAX 8192
 int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached,
                   const int *fresh, int *tables, int width, long ldt,

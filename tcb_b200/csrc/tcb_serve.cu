@@ -21,8 +21,22 @@ bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page =
 int log2i(int v) { return v <= 1 ? 0 : 1 + log2i(v / 2); }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// ------------------------------------------------------------ page plan
+// bytes of an array (none where n is 0)
+struct Span {
+  const void *p;
+  long n;
+  uintptr_t at() const { return reinterpret_cast<uintptr_t>(p); }
+};
+bool meet(const Span &a, const Span &b) { return a.n > 0 && b.n > 0 && a.at() < b.at() + b.n && b.at() < a.at() + a.n; }
+// whether a lies in one of `count` rows of `n` bytes, `step` apart
+bool meets_rows(const Span &a, const void *rows, int count, long n, long step) {
+  if (count < 1 || !meet(a, {rows, (count - 1) * step + n})) return false;
+  if (count == 1 || a.at() < reinterpret_cast<uintptr_t>(rows)) return true;
+  const long off = (long)(a.at() - reinterpret_cast<uintptr_t>(rows)) % step;  // from the start of its row
+  return off < n || off + a.n > step;
+}
 
+// ------------------------------------------------------------ page plan
 
 struct PlanArgs {
   int B, page, page_shift, width, free_cap, rows;
@@ -311,12 +325,24 @@ int tcb_page_plan(tcb_ctx *ctx, int B, int page, const int *cached, const int *f
   if (!row_start || !balance || !n_free || (B && (!cached || !fresh || !kv_len || (width && !tables))) ||
       (free_cap && !free_pages) || (rows && (!slots || !positions)))
     return TCB_ERR_NULL;
-  if (balance == n_free || taken == n_free) return TCB_ERR_UNSUPPORTED;  // the grid reads one while the other is written
   for (const void *p : {(const void *)cached, (const void *)fresh, (const void *)tables, (const void *)free_pages,
                         (const void *)n_free, (const void *)row_start, (const void *)kv_len, (const void *)positions,
                         (const void *)balance, (const void *)taken})
     if (!aligned(p, 4)) return TCB_ERR_ALIGN;
   if (!aligned(slots, 8)) return TCB_ERR_ALIGN;
+  // CTAs still read what others have read and CTA 0 or their neighbours write: no
+  // output lies in an input, in the tables' rows or in another output
+  const Span in[] = {{cached, 4l * B}, {fresh, 4l * B}, {free_pages, 4l * free_cap}, {n_free, 4}};
+  const Span out[] = {{row_start, 4 * (B + 1l)}, {kv_len, 4l * B}, {slots, 8l * rows}, {positions, 4l * rows}, {balance, 4}, {taken, taken ? 4 : 0}};
+  for (const Span &o : out) {
+    for (const Span &i : in)
+      if (meet(o, i)) return TCB_ERR_UNSUPPORTED;
+    for (const Span *p = out; p != &o; p++)
+      if (meet(o, *p)) return TCB_ERR_UNSUPPORTED;
+    if (meets_rows(o, tables, B, 4l * width, 4 * ldt)) return TCB_ERR_UNSUPPORTED;
+  }
+  for (const Span &i : in)
+    if (meets_rows(i, tables, B, 4l * width, 4 * ldt)) return TCB_ERR_UNSUPPORTED;
   int rc = tcb::ctx_bind(ctx);
   if (rc != TCB_OK) return rc;
   PlanArgs a{B, page, log2i(page), width, free_cap, rows, cached, fresh, tables, ldt, free_pages, n_free,
