@@ -59,13 +59,16 @@ struct PageAttnArgs {
 // Requests of many rows, and the shared prefix of a batch (a.prefix set: all
 // T rows against its positions): tcb_page_rows.cu.  With more than one CTA
 // along the positions, and for a prefix, the kernel leaves partial results
-// in scratch: o[split][T * H][head_dim] and, o_bytes on, (maximum, sum)
-// pairs [split][T * H]; a prefix's are joined by the kernel of its suffixes.
+// in scratch: o[split][prows * H][head_dim] and, o_bytes on, (maximum, sum)
+// pairs [split][prows * H], where prows is T, or B * max_rows (`each`) where that
+// is less; a prefix's are joined by the kernel of its suffixes.
 struct RowsPlan {
   int tiles, split;
   long items;   // pairs of query tiles that have CTAs (for each KV head and part)
   bool packed;  // counted over all requests
   bool partial;
+  int prows;
+  bool each;
   size_t o_bytes, bytes;
 };
 RowsPlan page_rows_plan(const PageAttnArgs &a);

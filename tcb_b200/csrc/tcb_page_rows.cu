@@ -71,7 +71,10 @@ struct Args {
   int split;           // CTAs along the positions
   int box;             // rows of a TMA box
   int joined;          // rows of q in one run (prefix): row index / G is the row of q
-  float *po;           // split or prefix: partial results [split][rows * H][HD]
+  int prows;           // rows with partial results: those of q, or, where q has more than the
+                       // requests can have (`each` then), max_rows for every request
+  bool each;
+  float *po;           // split or prefix: partial results [split][prows * H][HD]
   float2 *pml;         // and their (maximum, sum)
   CUtensorMap tk, tv;
 };
@@ -677,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
       const float l = (la.x + la.y) + (lb.x + lb.y);
       const bool empty = iters == 0 || m == -INFINITY;
       const float inv = p.po ? 1.f : __fdiv_rn(1.f, empty ? 1.f : l);
-      const long prow = ((long)part * a.T + r) * a.H + head;
+      const long prow = ((long)part * p.prows + (p.each ? (long)request * a.max_rows + xi : r)) * a.H + head;
       if (p.po && live) p.pml[prow] = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
       uint32_t ahead[32];  // the next 32 columns, on their way while these are written
       if (iters > 0 && ok) tmem_ld(to_addr, ahead);
@@ -758,28 +761,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_page_rows(const __grid_constant
 }
 
 // out = the partials of every split joined in order, for the rows of requests
-// (4 elements a thread; H * HD / 4 threads a row)
+// (4 elements a thread; H * HD / 4 threads a row; prows and each as in Args)
 template <int DT, int HD>
-__global__ void __launch_bounds__(256) k_rows_join(const PageAttnArgs a, int split, const float *po, const float2 *pml) {
+__global__ void __launch_bounds__(256) k_rows_join(const PageAttnArgs a, int split, int prows, bool each, const float *po, const float2 *pml) {
   mv::pdl_wait();
   mv::pdl_launch_dependents();
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = i / (HD / 4);
-  if (row >= (long)a.T * a.H) return;
+  const long row = i / (HD / 4), rows = (long)prows * a.H;
+  if (row >= rows) return;
   const int d = (int)(i - row * (HD / 4)) * 4;
-  const long r = row / a.H;
+  long r = row / a.H;
   const int head = (int)(row - r * a.H);
   // rows outside every request keep what they hold
   bool mine = false;
-  for (int b = 0; b < a.B && !mine; b++) mine = r >= a.row_start[b] && r < min(a.row_start[b + 1], max(a.row_start[b], 0) + a.max_rows);
+  if (each) {
+    const int b = (int)(r / a.max_rows), at = (int)(r - (long)b * a.max_rows), r0 = min(max(a.row_start[b], 0), a.T);
+    mine = at < min(a.row_start[b + 1], a.T) - r0;
+    r = r0 + at;
+  } else {
+    for (int b = 0; b < a.B && !mine; b++) mine = r >= a.row_start[b] && r < min(a.row_start[b + 1], max(a.row_start[b], 0) + a.max_rows);
+  }
   if (!mine) return;
   float top = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < split; s++) top = fmaxf(top, pml[(long)s * a.T * a.H + row].x);
+  for (int s = 0; s < split; s++) top = fmaxf(top, pml[s * rows + row].x);
   for (int s = 0; s < split; s++) {
-    const float2 ml = pml[(long)s * a.T * a.H + row];
+    const float2 ml = pml[s * rows + row];
     const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-    const float4 v = *reinterpret_cast<const float4 *>(po + ((long)s * a.T * a.H + row) * HD + d);
+    const float4 v = *reinterpret_cast<const float4 *>(po + (s * rows + row) * HD + d);
     acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
     sum += f * ml.y;
   }
@@ -810,8 +819,8 @@ cudaError_t launch(const Args &p, bool packed, dim3 grid, cudaStream_t s) {
   };
   cudaError_t e = packed ? go(std::integral_constant<bool, true>()) : go(std::integral_constant<bool, false>());
   if (e == cudaSuccess && p.po && !p.joined) {
-    const long n = (long)p.a.T * p.a.H * (HD / 4);
-    e = launch_serve(k_rows_join<DT, HD>, dim3((unsigned)((n + 255) / 256)), 256, 0, 1, s, p.a, p.split, p.po, p.pml);
+    const long n = (long)p.prows * p.a.H * (HD / 4);
+    e = launch_serve(k_rows_join<DT, HD>, dim3((unsigned)((n + 255) / 256)), 256, 0, 1, s, p.a, p.split, p.prows, p.each, p.po, p.pml);
   }
   return e;
 }
@@ -839,8 +848,11 @@ RowsPlan page_rows_plan(const PageAttnArgs &a) {
   pl.split = (int)std::max<long>(1, std::min<long>(148 / units, keys / 2));
   if (joined) pl.split = std::min(pl.split, kMaxPrefixParts);
   pl.partial = joined || pl.split > 1;
+  // a padded batch has rows of q outside every request: no room for theirs
+  pl.each = !joined && (long)a.B * a.max_rows < a.T;
+  pl.prows = pl.each ? a.B * a.max_rows : a.T;
   if (pl.partial) {
-    const size_t n = (size_t)pl.split * a.T * a.H;
+    const size_t n = (size_t)pl.split * pl.prows * a.H;
     pl.o_bytes = n * a.kv.head_dim * sizeof(float);
     pl.bytes = pl.o_bytes + n * sizeof(float2);
   }
@@ -855,6 +867,8 @@ int launch_page_rows(tcb_ctx *ctx, const PageAttnArgs &a, const RowsPlan &pl, vo
   p.split = pl.split;
   p.joined = a.prefix != nullptr;
   p.box = std::min(a.kv.page, pr::kKeys);
+  p.prows = pl.prows;
+  p.each = pl.each;
   if (pl.partial) {
     p.po = static_cast<float *>(scratch);
     p.pml = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + pl.o_bytes);
