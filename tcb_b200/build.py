@@ -4,10 +4,12 @@ _tcb_torch.so (its serving entry points for torch tensors) with g++.
     python -m tcb_b200.build          # or tcb_b200.build.build()
 
 The libraries land next to this file (tcb_b200/libtcb.so, _tcb_torch.so) so they
-travel with the source tree; nothing is installed into site-packages.
+travel with the source tree; nothing is installed into site-packages.  libtcb.so
+needs nvcc alone: without torch it is built and _tcb_torch.so is left out.
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
@@ -35,6 +37,35 @@ def _stale(objs, deps) -> bool:
     return any(os.path.getmtime(o) < newest for o in objs)
 
 
+def _torch_command():
+    """The compiler's command for _tcb_torch.so; None without torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    t = list(spec.submodule_search_locations)[0]
+    return [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
+            "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(t, "include"), "-isystem",
+            os.path.join(t, "include", "torch", "csrc", "api", "include"), "-isystem", "/usr/local/cuda/include",
+            os.path.join(CSRC, "tcb_torch.cpp"), "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_cuda",
+            "-ltorch_cpu", "-ltorch_python"]
+
+
+def _torch_stamp() -> str:
+    """What _tcb_torch.so was built against: the Python and torch it only works with."""
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        version = "?"
+    return f"{sys.version} torch {version}\n"
+
+
+def _read(path: str) -> str:
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read()
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     bdir = os.path.join(HERE, "_build")
     os.makedirs(bdir, exist_ok=True)
@@ -48,14 +79,11 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if force or _stale([o], [s] + headers):
             cmds.append([NVCC, *ARCH, *FLAGS, "-c", s, "-o", o])
 
-    torch_src = os.path.join(CSRC, "tcb_torch.cpp")
-    if force or _stale([TORCH_LIB], [torch_src, headers[-1]]):
-        t = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
-        cmds.append([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
-                     "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(t, "include"), "-isystem",
-                     os.path.join(t, "include", "torch", "csrc", "api", "include"), "-isystem", "/usr/local/cuda/include",
-                     torch_src, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
-                     "-ltorch_python"])
+    torch_cmd, stamp = _torch_command(), os.path.join(bdir, "tcb_torch.stamp")
+    if torch_cmd is None:
+        print("torch is not installed: _tcb_torch.so (tcb_b200.serve) is left out", file=sys.stderr, flush=True)
+    elif force or _stale([TORCH_LIB], [os.path.join(CSRC, "tcb_torch.cpp"), headers[-1]]) or _read(stamp) != _torch_stamp():
+        cmds.append(torch_cmd)
 
     def compile_one(cmd):
         if verbose:
@@ -66,6 +94,9 @@ def build(verbose: bool = False, force: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=max(1, min(len(cmds), os.cpu_count() or 1))) as ex:
         for f in [ex.submit(compile_one, c) for c in cmds]:
             f.result()
+    if torch_cmd in cmds:
+        with open(stamp, "w") as f:
+            f.write(_torch_stamp())
     if force or _stale([LIB], objs):
         cmd = [NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB, *objs]
         if verbose:
