@@ -352,7 +352,8 @@ typedef struct tcb_kv_pages {
  *              row_start[B] get -1
  *   balance    [1]      n less need[0] + .. + need[b] of the last request b that is not
  *              refused: the free pages left, or, below 0, how many the requests
- *              refused before it lacked
+ *              refused before it lacked (not the height of the stack: that is
+ *              n - taken)
  *   taken      [1] or NULL  pages taken from the end of the free list
  * A request is refused, with kv_len 0 and its rows' slots and positions -1,
  * when a length of it is negative, its table (width entries, rows ldt apart)
@@ -385,7 +386,8 @@ int tcb_kv_append(tcb_ctx *ctx, const tcb_kv_pages *kv, int T, const void *k,
  * p = kv_len[b] - (row_start[b+1] - row_start[b]) + i and sees
  *   j <= p  with  j > p - window  or  j < sinks    (window < 0: every j <= p).
  * Query head h reads KV head h / (H / n_kv_heads).  A row that sees nothing
- * (p < 0, or window 0 without sinks) gives zeros; what the cache holds where
+ * (p < 0, or window 0 without sinks) gives zeros, as does one whose scores are
+ * all -inf, and a score of +inf or NaN makes its row NaN; what the cache holds where
  * a row does not look, NaN included, does not reach its result.
  *   q, out     T rows of H heads of head_dim elements in the cache's type, ldq
  *              and ldo elements apart; 16-byte aligned rows
@@ -410,8 +412,8 @@ int tcb_page_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int T, int H,
  *   out[b, h] = softmax over j < kv_len[b] of scale * q[b, h] . k[j], times v
  * with positions j < prefix_len read from the pages prefix[j / page] (device,
  * ceil(prefix_len / page) page numbers), once for all requests where that is
- * faster (long prefixes, many requests), and the others from tables[b][j / page] as in tcb_page_attn (entries of whole
- * prefix pages are not read).  kv_len[b] may be below prefix_len; 0 gives
+ * faster (long prefixes, many requests), and the others from tables[b][j / page]
+ * as in tcb_page_attn (entries of whole prefix pages are not read).  kv_len[b] may be below prefix_len; 0 gives
  * zeros. */
 int tcb_prefix_attn(tcb_ctx *ctx, const tcb_kv_pages *kv, int B, int H,
                     const void *q, long ldq, void *out, long ldo,

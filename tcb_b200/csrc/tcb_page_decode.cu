@@ -13,9 +13,14 @@
 // far inside f16's range), so the usual 16 positions cost no maximum across
 // lanes and no rescaling.
 //
+// Roundings: the weights, to the cache's type, are what the second product takes;
+// the sum is of the rounded weights, whose errors then cancel in part.  Against 64
+// bits a call errs by 2.1e-4 (f16) to 2.2e-3 (bf16), where one rounding of the
+// result errs by 2.1e-4 and 1.7e-3.
+//
 // Bound: the K/V bytes, each read once: 3.63 GB for 64 sequences of up to 32768
-// positions (window 16384, 8 KV heads of 128, bf16) in 555 us = 6540 GB/s, the
-// copy rate.  Layout:
+// positions (window 16384, 8 KV heads of 128, bf16) in 555 to 570 us = 6370 to 6540
+// GB/s, the copy rate.  Layout:
 // every fragment comes straight from global memory into registers, without
 // shared memory: the k slots of S^T are dealt so that a lane's A fragments of
 // K are 16-byte pieces of one position (lane (g, t): positions g and g + 8,
@@ -74,7 +79,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 // CTAs of 4 warps per SM that leave a thread the registers it needs without spills (168
-// and 236 at head_dim 128).  At batch 64 with 3 CTAs: 554 us against 595 with
+// and 234 at head_dim 128).  At batch 64 with 3 CTAs: 554 us against 595 with
 // 4 and 128 spilling registers.
 template <int HD, int NT>
 constexpr int kCtas = (NT == 1 ? 4 : 3) - (HD == 128);
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? kCtas<HD, NT> : 1) 
 
   // behind the prefix's kernel too: what the kernels before that one wrote (lengths,
   // pages, K/V rows) is promised to a grid that has waited itself.  (Reading the
-  // suffixes beside the prefix's tiles took 85.6 us where this takes 87.5, 64
+  // suffixes beside the prefix's tiles took 85.6 us where this takes 87.3, 64
   // requests behind 16384 positions.)
   mv::pdl_launch_dependents();  // before the wait: 7.3 us for one sequence, 7.6 after it
   mv::pdl_wait();

@@ -10,6 +10,10 @@
 // to the cache's type and written over S, and O += P V with O in tensor
 // memory.  O is rescaled only when a row's maximum has grown by more than
 // 2^kSlack (weights up to 2^kSlack are far inside f16's range, sums are f32).
+// The tensor cores take P in the cache's type only; the sum is of the weights
+// before that rounding (after it each would have to be unpacked).  Against 64 bits a
+// call errs by 2.8e-4 (f16) and 2.2e-3 (bf16), where one rounding of the result
+// errs by 2.1e-4 and 1.6e-3.
 //
 // Bound: at 128 elements a head a tile costs 1024 tensor cycles (S and P V)
 // and 16384 exponentials, 1024 cycles of the SM's 16 a cycle: both pipes are
@@ -17,8 +21,11 @@
 // warp for both keeps them in turn (with one each they fall into step: 560 us
 // where this took 465).
 // Measured: 8192 rows, 32 heads on 8 KV heads of 128, window 4096, bf16: 401 us =
-// 1030 TFLOP/s, 0.63 of the cuBLAS burst rate; 1.85 us per pair of tiles and 128
-// positions, and 11 of a CTA's 72 us at its start and end.
+// 1030 TFLOP/s, 0.63 of the cuBLAS burst rate, at full clocks;
+// 436 to 448 us = 920 to 950 TFLOP/s in a loop of such calls, 0.65 to 0.67 of cuBLAS
+// under the power limit.  1.85 us per pair of tiles and 128 positions, and 11 of a CTA's
+// 72 us at its start and end.  168 registers a thread, with 56 to 60 bytes
+// spilled.
 //
 //   warp 0      K and V tiles by TMA from the pages (128-byte swizzle; one box
 //               per page and 64 elements, one lane each), 2 stages of each

@@ -12,8 +12,9 @@ One step of a batch of requests:
   penalize(...)         penalties, biases and masks on the logits, the pick
 All lengths and page numbers are int32 tensors on the device; nothing here
 waits for the device.  Every call runs on `stream` (the current one when it is
-None), and calls on one context are to be ordered on one stream.  Device-side
-findings (a page outside the pool, a length past max_len) are read with
+None), and calls on one context are to be ordered on one stream; tensors given
+to another stream than their own are the caller's to keep until it is done.
+Device-side findings (a page outside the pool, a length past max_len) are read with
 Context.device_error().
 """
 from __future__ import annotations
@@ -94,8 +95,11 @@ def plan(ctx, page, cached, fresh, tables, free, n_free, row_start, kv_len, slot
     """tcb_page_plan: cached and fresh int32 [B]; tables int32 [B, width]
     (extended in place); free int32, the stack of free pages, of which the
     first n_free[0] are free; written: row_start int32 [B + 1], kv_len int32
-    [B], slots int64 and positions int32 [rows], balance int32 [1] (the free
-    pages left, below 0 the shortage), taken int32 [1] or None (pages taken)."""
+    [B], slots int64 and positions int32 [rows], taken int32 [1] or None (the
+    pages taken, by which the caller lowers n_free) and balance int32 [1] (n_free
+    less taken; or, below 0, the pages that were short, where a request that lacks
+    none is served behind refused ones).  A refused request has kv_len 0.  Outputs
+    that overlap an input, the tables or one another raise TcbError."""
     rc = _view().plan(ctx.handle.value, ctx.device, page, cached, fresh, tables, free, n_free, row_start, kv_len, slots,
                       positions, balance, taken, stream)
     if rc:
